@@ -701,6 +701,78 @@ int mdb_window_attn(const mdb_window_attn_args* args, mdb_stream_t stream);
 int mdb_pick_token(const float* logits, int64_t ld, int m, int vocab, const float* temperatures, uint32_t seed,
                    const uint32_t* step_dev, int64_t* out, uint32_t* status_out, mdb_stream_t stream);
 
+/* ---- long contexts: rotary positions, a shared prefix, weights of the keys, eviction --------------------
+ * (No counterparts in the reference, whose decoder rotates over the whole head without scaling and keeps every key;
+ * NV/layers/rotary_embedding.py:6-48, NV/layers/attention.py:10-40.)  Caches are [num_pages][256][hkv][...] as above; a
+ * length beyond what its page table (rows of table_pages entries, table_stride apart) or a row of weights can address is cut to
+ * it, with MDB_STATUS_BAD_PAGE. */
+
+/* Rotary positions without a norm: with t = positions[row] * inv_freq[i] the channel pair (i, i + rot_dims / 2) of a head, or
+ * with `interleaved` (2 i, 2 i + 1), becomes scale * (a cos t - b sin t, b cos t + a sin t); `inverse` turns by -t (the
+ * gradient with respect to the input is the inverse turn of the gradient).  Channels from rot_dims on pass as they come.  Rows
+ * and heads lie *_row and *_head elements apart; outputs may be the inputs.  With slots (int32 [n], -1: skipped) the keys, and
+ * the values v as they come (NULL: none), go to rows of the contiguous caches [num_slots][kv_heads][dim] and k_out is
+ * not used; without slots v must be NULL.  kv_heads 0: queries alone. */
+typedef struct {
+  int32_t dtype, n, heads, kv_heads, dim, rot_dims, interleaved, inverse;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int64_t* positions;
+  const double* inv_freq;
+  const int32_t* slots;
+  int64_t num_slots;
+  void* q_out;
+  void* k_out;
+  int64_t q_out_row, q_out_head, k_out_row, k_out_head;
+  void* k_cache;
+  void* v_cache;
+  float scale;
+} mdb_rotary_embed_args;
+int mdb_rotary_embed(const mdb_rotary_embed_args* args, mdb_stream_t stream);
+
+/* Block attention of a batch whose requests share a prefix: as mdb_attn_block_paged, but every query row sees the prefix_len[0]
+ * keys of the pages in prefix_table (once, for all requests) and then keys [0, ctx_lens[b]) of its request's own pages.
+ * lse (may be NULL) [bs][block][hq] = the natural logarithm of the softmax's denominator.  A row without any key gets zeros and
+ * -inf.  prefix_pages 0: no prefix (prefix_table and prefix_len may be NULL).  The workspace is always needed; calls in flight at
+ * the same time need one each. */
+int64_t mdb_attn_shared_workspace_bytes(int bs, int block, int hq, int hkv);
+int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int32_t* prefix_table,
+                          int prefix_pages, const int32_t* prefix_len, const int32_t* block_table, int table_stride,
+                          int table_pages, const int32_t* ctx_lens, int bs, int block, int hq, int hkv, int num_pages,
+                          float softmax_scale, void* workspace, int64_t workspace_bytes, mdb_stream_t stream);
+
+/* The weight every key of a request's own pages receives from a block of queries, by key head: out[b][h][j] = decay *
+ * previous[b][h][j] + the sum over the block's tokens t and the heads g of group h of exp(q . k_j * softmax_scale -
+ * lse[b][t][g]) for j < ctx_lens[b], 0 behind.  lse as mdb_attn_block_shared returns it (rows of -inf weigh nothing).  out and
+ * previous (may be NULL: 0; may be out) fp32 [bs][hkv][cols]. */
+int mdb_key_weights(const void* q, const void* k_cache, const float* lse, const int32_t* block_table, int table_stride,
+                    int table_pages, const int32_t* ctx_lens, int bs, int block, int hq, int hkv, int num_pages, float softmax_scale,
+                    const float* previous, float decay, float* out, int64_t cols, mdb_stream_t stream);
+
+/* Eviction: of the seqlens[b] keys of a request the last `recent` and, by key head, the budget - recent of largest weight among those
+ * in front stay (NaN counts as the lowest weight; the lowest index wins a tie); all of them where there are no more than budget.
+ * Their rows of row_bytes bytes (a multiple of 16) in K and V, and their weights, move in order to the first places of the
+ * request's pages (out_table NULL) or of the pages in out_table, which hold none of those read.  Pages that are written
+ * belong to one request.  kept [bs][kv_heads][budget] = old places, -1 behind the last; weights_out (may be NULL, may be
+ * weights) gets 0 there; seqlens_out (may be seqlens) = min(seqlens, budget). */
+typedef struct {
+  int32_t bs, kv_heads, row_bytes, budget, recent, num_pages, table_stride, table_pages, out_table_stride, out_table_pages;
+  void* k_cache;
+  void* v_cache;
+  const float* weights;
+  int64_t weight_row, weight_head, weight_cols;
+  float* weights_out;
+  int64_t weight_out_row, weight_out_head;
+  const int32_t* seqlens;
+  int32_t* seqlens_out;
+  const int32_t* block_table;
+  const int32_t* out_table;
+  int32_t* kept;
+} mdb_kv_evict_args;
+int mdb_kv_evict(const mdb_kv_evict_args* args, mdb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,6 +81,18 @@ MoeRouteArgs = _struct("MoeRouteArgs", [(n, _i) for n in ("m", "experts", "top",
     ("logits", Rows), ("row_slot", _p), ("ids", _p), ("weights", _p)])
 MoePlanArgs = _struct("MoePlanArgs", [(n, _i) for n in ("m", "top", "experts", "max_tiles")] + [
     ("ids", _p), ("slot", _p), ("row_token", _p), ("tile_expert", _p), ("num_tiles", _p)])
+RotaryEmbedArgs = _struct("RotaryEmbedArgs", [(n, _i) for n in (
+    "dtype", "n", "heads", "kv_heads", "dim", "rot_dims", "interleaved", "inverse")] + [
+    ("q", _p), ("k", _p), ("v", _p), ("q_row", _i64), ("q_head", _i64), ("k_row", _i64), ("k_head", _i64), ("v_row", _i64),
+    ("v_head", _i64), ("positions", _p), ("inv_freq", _p), ("slots", _p), ("num_slots", _i64), ("q_out", _p), ("k_out", _p),
+    ("q_out_row", _i64), ("q_out_head", _i64), ("k_out_row", _i64), ("k_out_head", _i64), ("k_cache", _p), ("v_cache", _p),
+    ("scale", _f)])
+KvEvictArgs = _struct("KvEvictArgs", [(n, _i) for n in (
+    "bs", "kv_heads", "row_bytes", "budget", "recent", "num_pages", "table_stride", "table_pages", "out_table_stride",
+    "out_table_pages")] + [
+    ("k_cache", _p), ("v_cache", _p), ("weights", _p), ("weight_row", _i64), ("weight_head", _i64), ("weight_cols", _i64),
+    ("weights_out", _p), ("weight_out_row", _i64), ("weight_out_head", _i64), ("seqlens", _p), ("seqlens_out", _p),
+    ("block_table", _p), ("out_table", _p), ("kept", _p)])
 
 # name -> (restype, argtypes); mirrors include/mdb200.h one to one
 SIGNATURES = {
@@ -155,6 +167,11 @@ SIGNATURES = {
     "mdb_latent_attn": (_i, [_i, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _f, _i, _p, _i64, _p]),
     "mdb_gather_latents": (_i, [_i, _p, _p, _i, _i, _p, _i, _i, _p, _i, _p]),
     "mdb_attn_causal_varlen": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i, _i, _i64, _i64, _i, _i, _f, _p]),
+    "mdb_rotary_embed": (_i, [C.POINTER(RotaryEmbedArgs), _p]),
+    "mdb_attn_shared_workspace_bytes": (_i64, [_i, _i, _i, _i]),
+    "mdb_attn_block_shared": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _i, _i, _p, _i, _i, _i, _i, _i, _f, _p, _i64, _p]),
+    "mdb_key_weights": (_i, [_p, _p, _p, _p, _i, _i, _p, _i, _i, _i, _i, _i, _f, _p, _f, _p, _i64, _p]),
+    "mdb_kv_evict": (_i, [C.POINTER(KvEvictArgs), _p]),
     "mdb_pick_token": (_i, [_p, _i64, _i, _i, _p, _u32, _p, _p, _p, _p]),
 }
 

@@ -6,6 +6,7 @@ and none has a fallback.
 """
 from __future__ import annotations
 
+import math
 
 import torch
 
@@ -903,3 +904,242 @@ def copy_rows(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor) -> torc
     t, o = (table, out) if table.dtype == _BF16 else (table.view(_BF16), out.view(_BF16))
     gather_rows(t, ids, out=o)
     return out
+
+
+# --------------------------------------------------------------------------
+# Long contexts: rotary positions of any layout and scaling, attention behind a shared prefix, the weights of its keys and the
+# eviction that goes by them.
+
+def _here(**tensors) -> None:
+    """All tensors (None: absent) on the current CUDA device: kernels are launched there."""
+    dev = torch.cuda.current_device() if _device is None else None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor (libmdb200 has no CPU path)")
+        if dev is None:
+            dev = _device()
+        if t.get_device() != dev:
+            raise RuntimeError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{dev}")
+
+
+def rope_frequencies(rot_dims: int, base: float = 10000.0, scaling: dict | None = None, device="cuda") -> tuple[torch.Tensor, float]:
+    """(frequencies float64 [rot_dims / 2], factor on the rotated channels) for ``rotary_embed``.
+
+    ``scaling`` draws the positions out for contexts of ``factor`` times the length the weights were trained with: {"type": "linear",
+    "factor": s} divides every frequency by s; "ntk" raises the base to base * s^(r / (r - 2)); "yarn" (with
+    "original_max_position", "beta_fast" 32, "beta_slow" 1) divides the frequencies that make fewer than beta_slow turns over the
+    original length, keeps those that make more than beta_fast, blends the others by their index, and gives the factor
+    0.1 ln s + 1 ("attention_factor" overrides it)."""
+    if rot_dims < 2 or rot_dims % 2:
+        raise ValueError("rot_dims must be even and positive")
+    kind = None if scaling is None else scaling.get("type")
+    if kind not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown rotary scaling {kind!r}: linear, ntk or yarn")
+    s = 1.0 if kind is None else float(scaling["factor"])
+    if not s >= 1.0:
+        raise ValueError("the scaling factor must be at least 1")
+    if kind == "ntk":
+        if rot_dims == 2:
+            raise ValueError("ntk scaling needs more than one frequency")
+        base = base * s ** (rot_dims / (rot_dims - 2))
+    f = [base ** (-2.0 * i / rot_dims) for i in range(rot_dims // 2)]
+    factor = 1.0
+    if kind == "linear":
+        f = [x / s for x in f]
+    elif kind == "yarn":
+        length = float(scaling["original_max_position"])
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+
+        def index(turns):       # of the frequency that makes so many turns over the original length
+            return rot_dims * math.log(length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        lo, hi = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rot_dims - 1)
+        for i, x in enumerate(f):
+            scaled = min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0)
+            f[i] = x / s * scaled + x * (1.0 - scaled)
+        factor = float(scaling.get("attention_factor") or 0.1 * math.log(s) + 1.0)
+    return torch.tensor(f, dtype=torch.float64, device=device), factor
+
+
+def _heads_of(t: torch.Tensor, n: int, d: int, dtype, name: str) -> int:
+    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != d or t.stride(2) != 1 or t.dtype != dtype:
+        raise ValueError(f"{name} must be [{n}, heads, {d}] of {dtype} with a dense last dimension")
+    return t.shape[1]
+
+
+def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
+                 scale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                 v: torch.Tensor | None = None, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+                 slot_mapping: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of queries [n, hq, d] and keys [n, hkv, d] (bf16 or fp32, row and head strides free), without the norms of
+    ``qknorm_rope_commit``: the first ``2 * len(inv_freq)`` channels turn in pairs (i, i + r/2), or (2 i, 2 i + 1) with
+    ``interleaved``, by positions (int64 [n]) times ``inv_freq`` (float64) and are multiplied by ``scale``; the others pass.
+    ``inverse`` turns back, which is also the gradient with respect to the input.  ``q_out`` / ``k_out`` may be the inputs.
+    With ``slot_mapping`` (int32 [n], -1 = skip) the keys, and ``v`` if given, go to those rows of the caches [pages, 256, hkv, d]
+    as ``store_kvcache`` puts them there.  Returns (q_out, k_out or None)."""
+    if q.dim() != 3:
+        raise ValueError("q must be [n, heads, dim]")
+    n, hq, d = q.shape
+    _here(q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, q_out=q_out, k_out=k_out, k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
+    dtype = _act_dtype(q, "q")
+    _heads_of(q, n, d, q.dtype, "q")
+    if positions.dtype != torch.int64 or positions.numel() != n or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int64 tensor with one entry per row")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > d:
+        raise ValueError("inv_freq must be a contiguous float64 vector of at most half as many entries as a head has channels")
+    if q_out is None:
+        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    elif _heads_of(q_out, n, d, q.dtype, "q_out") != hq:
+        raise ValueError("q_out must have the shape of q")
+    hkv = 0 if k is None else _heads_of(k, n, d, q.dtype, "k")
+    a = _lib.RotaryEmbedArgs(dtype, n, hq, hkv, d, 2 * inv_freq.numel(), int(interleaved), int(inverse))
+    a.q, a.q_row, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
+    a.q_out, a.q_out_row, a.q_out_head = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    a.positions, a.inv_freq, a.scale = positions.data_ptr(), inv_freq.data_ptr(), scale
+    if slot_mapping is not None:
+        if k is None or k_cache is None or (v is None) != (v_cache is None) or k_out is not None:
+            raise ValueError("a store needs k and k_cache, v and v_cache together, and no k_out")
+        if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != n or not slot_mapping.is_contiguous():
+            raise ValueError("slot_mapping must be a contiguous int32 tensor with one entry per row")
+        for c, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            if c is not None and (c.dim() != 4 or c.shape[2] != hkv or c.shape[3] != d or c.dtype != q.dtype or not c.is_contiguous()):
+                raise ValueError(f"{nm} must be contiguous [pages, 256, {hkv}, {d}] of {q.dtype}")
+        if v is not None:
+            if _heads_of(v, n, d, q.dtype, "v") != hkv or v_cache.shape != k_cache.shape:
+                raise ValueError("v must have the shape of k, and the caches the same shape")
+            a.v, a.v_row, a.v_head, a.v_cache = v.data_ptr(), v.stride(0), v.stride(1), v_cache.data_ptr()
+        a.slots, a.num_slots, a.k_cache = slot_mapping.data_ptr(), k_cache.shape[0] * k_cache.shape[1], k_cache.data_ptr()
+    elif v is not None or k_cache is not None or v_cache is not None:
+        raise ValueError("v and the caches go with a slot_mapping")
+    elif k is not None:
+        if k_out is None:
+            k_out = torch.empty((n, hkv, d), dtype=q.dtype, device=q.device)
+        elif _heads_of(k_out, n, d, q.dtype, "k_out") != hkv:
+            raise ValueError("k_out must have the shape of k")
+        a.k_out, a.k_out_row, a.k_out_head = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+    if k is not None:
+        a.k, a.k_row, a.k_head = k.data_ptr(), k.stride(0), k.stride(1)
+    _lib.check(_lib.lib().mdb_rotary_embed(a, _stream()), "mdb_rotary_embed")
+    return q_out, k_out
+
+
+def shared_prefix_workspace_bytes(bs: int, block: int, hq: int, hkv: int) -> int:
+    """Scratch bytes of ``block_attn_shared_prefix``."""
+    return int(_lib.lib().mdb_attn_shared_workspace_bytes(bs, block, hq, hkv))
+
+
+def block_attn_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_seqlen: torch.Tensor | None,
+                             prefix_table: torch.Tensor | None, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                             softmax_scale: float | None = None, workspace: torch.Tensor | None = None,
+                             out: torch.Tensor | None = None, want_lse: bool = False, lse: torch.Tensor | None = None):
+    """``block_attn_with_kvcache`` for a batch whose requests share a prefix: every query of q [bs, B, Hq, 128] sees the
+    ``prefix_seqlen`` (int32 [1]) keys of the pages ``prefix_table`` (int32 [pages]) and then the ``cache_seqlens[b]`` keys of its
+    request's pages.  The prefix is read and multiplied once for all requests.  None, None: no prefix.  A row that sees no key
+    gets zeros.  Returns out, or (out, lse) with ``want_lse`` or ``lse`` (fp32 [bs, B, Hq], the logarithm of the softmax's
+    denominator, -inf where there is no key): what ``key_weights`` takes.  Calls in flight at the same time need a ``workspace``
+    (``shared_prefix_workspace_bytes``) each."""
+    _here(q=q, k_cache=k_cache, v_cache=v_cache, prefix_seqlen=prefix_seqlen, prefix_table=prefix_table, cache_seqlens=cache_seqlens,
+          block_table=block_table, workspace=workspace, out=out, lse=lse)
+    bs, block, hq, hkv, pages, d = _block_attn_args(q, k_cache, v_cache, cache_seqlens, block_table, out)
+    prefix_pages = 0
+    if (prefix_table is None) != (prefix_seqlen is None):
+        raise ValueError("prefix_seqlen and prefix_table go together")
+    if prefix_table is not None:
+        prefix_pages = prefix_table.numel()
+        if prefix_table.dtype != torch.int32 or not prefix_table.is_contiguous():
+            raise ValueError("prefix_table must be a contiguous int32 list of pages")
+        if prefix_seqlen.dtype != torch.int32 or prefix_seqlen.numel() != 1:
+            raise ValueError("prefix_seqlen must be one int32")
+    if softmax_scale is None:
+        softmax_scale = d ** -0.5
+    if out is None:
+        out = torch.empty_like(q)
+    if lse is None:
+        lse = torch.empty((bs, block, hq), dtype=torch.float32, device=q.device) if want_lse else None
+    elif lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous fp32 [bs, block, Hq]")
+    need = _lib.lib().mdb_attn_shared_workspace_bytes(bs, block, hq, hkv)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _lib.check(_lib.lib().mdb_attn_block_shared(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(prefix_table), prefix_pages, _ptr(prefix_seqlen),
+        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cache_seqlens.data_ptr(), bs, block, hq, hkv, pages, float(softmax_scale),
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()), "mdb_attn_block_shared")
+    return out if lse is None else (out, lse)
+
+
+def key_weights(q: torch.Tensor, k_cache: torch.Tensor, lse: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                softmax_scale: float | None = None, previous: torch.Tensor | None = None, decay: float = 1.0,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """The attention weight every key of the requests' own pages has received: out[b, h, j] (fp32 [bs, Hkv, columns]) = decay *
+    previous[b, h, j] + the sum over the block's tokens and the query heads of group h of exp(q . k_j * softmax_scale - lse), for
+    j < cache_seqlens[b]; 0 behind.  ``lse`` is what the attention over all keys returned (``block_attn_shared_prefix``); q and the
+    caches as there.  For a prefix's keys, pass the batch as one request: q.view(1, bs * B, Hq, 128), its table and length.
+    ``previous`` may be ``out``; without either there are as many columns as the page table addresses."""
+    _here(q=q, k_cache=k_cache, lse=lse, cache_seqlens=cache_seqlens, block_table=block_table, previous=previous, out=out)
+    bs, block, hq, hkv, pages, d = _block_attn_args(q, k_cache, k_cache, cache_seqlens, block_table, None)
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous fp32 [bs, block, Hq]")
+    cols = block_table.shape[1] * 256 if out is None and previous is None else (previous if out is None else out).shape[-1]
+    for t, nm in ((previous, "previous"), (out, "out")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (bs, hkv, cols) or not t.is_contiguous()):
+            raise ValueError(f"{nm} must be contiguous fp32 [{bs}, {hkv}, {cols}]")
+    if out is None:
+        out = torch.empty((bs, hkv, cols), dtype=torch.float32, device=q.device)
+    _lib.check(_lib.lib().mdb_key_weights(
+        q.data_ptr(), k_cache.data_ptr(), lse.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        cache_seqlens.data_ptr(), bs, block, hq, hkv, pages, float(d ** -0.5 if softmax_scale is None else softmax_scale), _ptr(previous), float(decay), out.data_ptr(), cols, _stream()),
+        "mdb_key_weights")
+    return out
+
+
+def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                  budget: int, recent: int = 0, out_table: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
+                  seqlens_out: torch.Tensor | None = None, kept: torch.Tensor | None = None):
+    """Cuts every request's cache (one layer: [pages, 256, Hkv, d], bf16 or fp32) to ``budget`` keys per key head: the last ``recent``
+    stay, and of those in front the ones with the largest ``weights`` (fp32 [bs, Hkv, columns]; NaN counts as the lowest, the
+    lowest index wins a tie).  The rows of K and V that stay are packed in order into the first places of the request's pages, or
+    of the pages in ``out_table`` (int32 [bs, pages], none of the pages read: for pages that others still read, as a shared
+    prefix's); written pages must belong to one request.  Returns (kept int32 [bs, Hkv, budget] = old places, -1 behind the last;
+    new lengths int32 [bs]; weights of the kept keys [bs, Hkv, >= budget], 0 behind the last).  ``weights_out`` may be ``weights`` and
+    ``seqlens_out`` may be ``cache_seqlens``."""
+    _here(k_cache=k_cache, v_cache=v_cache, weights=weights, cache_seqlens=cache_seqlens, block_table=block_table, out_table=out_table,
+          weights_out=weights_out, seqlens_out=seqlens_out, kept=kept)
+    _act_dtype(k_cache, "k_cache")
+    if k_cache.dim() != 4 or k_cache.shape[1] != 256 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("the caches must be [pages, 256, Hkv, dim] of one type and shape")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    pages, _, hkv, d = k_cache.shape
+    if weights.dim() != 3 or weights.dtype != torch.float32 or weights.shape[1] != hkv or weights.stride(2) != 1:
+        raise ValueError("weights must be fp32 [bs, Hkv, columns] with a dense last dimension")
+    bs = weights.shape[0]
+    if not 0 <= recent <= budget or budget < 1:
+        raise ValueError("budget must be positive and recent between 0 and budget")
+    for t, nm in ((block_table, "block_table"), (out_table, "out_table")):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] < bs or (t.shape[1] > 1 and t.stride(1) != 1)):
+            raise ValueError(f"{nm} must be int32 [bs, pages per request] with unit stride inside a row")
+    if out_table is not None and out_table.shape[1] * 256 < min(budget, block_table.shape[1] * 256):
+        raise ValueError("out_table must have pages for budget keys")
+    for t, nm in ((cache_seqlens, "cache_seqlens"), (seqlens_out, "seqlens_out")):
+        if t is not None and (t.dtype != torch.int32 or t.numel() < bs or not t.is_contiguous()):
+            raise ValueError(f"{nm} must hold one contiguous int32 per request")
+    if weights_out is None:
+        weights_out = torch.empty((bs, hkv, budget), dtype=torch.float32, device=weights.device)
+    elif weights_out.dim() != 3 or weights_out.dtype != torch.float32 or weights_out.shape[:2] != (bs, hkv) or weights_out.shape[2] < budget or weights_out.stride(2) != 1:
+        raise ValueError("weights_out must be fp32 [bs, Hkv, at least budget] with a dense last dimension")
+    if seqlens_out is None:
+        seqlens_out = torch.empty(bs, dtype=torch.int32, device=weights.device)
+    if kept is None:
+        kept = torch.empty((bs, hkv, budget), dtype=torch.int32, device=weights.device)
+    elif kept.shape != (bs, hkv, budget) or kept.dtype != torch.int32 or not kept.is_contiguous():
+        raise ValueError("kept must be contiguous int32 [bs, Hkv, budget]")
+    a = _lib.KvEvictArgs(bs, hkv, d * k_cache.element_size(), budget, recent, pages, block_table.stride(0), block_table.shape[1],
+                         0 if out_table is None else out_table.stride(0), 0 if out_table is None else out_table.shape[1],
+                         k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2],
+                         weights_out.data_ptr(), weights_out.stride(0), weights_out.stride(1), cache_seqlens.data_ptr(), seqlens_out.data_ptr(),
+                         block_table.data_ptr(), _ptr(out_table), kept.data_ptr())
+    _lib.check(_lib.lib().mdb_kv_evict(a, _stream()), "mdb_kv_evict")
+    return kept, seqlens_out, weights_out

@@ -1,0 +1,122 @@
+"""Long-context operators, what the host decides: frequencies, workspace sizes, refusals.  No GPU calls."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def built():
+    import importlib
+    import __graft_entry__ as entry
+    entry.build()
+    return importlib.import_module("mineru-diffusion_b200")
+
+
+def freq(built, *args, **kw):
+    f, factor = built.ops.rope_frequencies(*args, device="cpu", **kw)
+    assert f.dtype == torch.float64
+    return f, factor
+
+
+def test_frequencies(built):
+    plain, factor = freq(built, 128, 10000.0)
+    assert factor == 1.0 and plain.shape == (64,)
+    assert torch.allclose(plain, 10000.0 ** (-torch.arange(0, 128, 2, dtype=torch.float64) / 128), rtol=1e-15)
+    linear, _ = freq(built, 128, 10000.0, scaling={"type": "linear", "factor": 4})
+    assert torch.equal(linear, plain / 4)
+    # the raised base keeps the fastest and divides the slowest by the factor
+    ntk, _ = freq(built, 128, 10000.0, scaling={"type": "ntk", "factor": 4})
+    assert ntk[0] == 1.0 and math.isclose(float(ntk[-1]), float(plain[-1]) / 4, rel_tol=1e-12)
+
+
+def test_frequencies_by_parts(built):
+    length, s = 4096, 8.0
+    plain, _ = freq(built, 64, 10000.0)
+    f, factor = freq(built, 64, 10000.0, scaling={"type": "yarn", "factor": s, "original_max_position": length})
+    assert math.isclose(factor, 0.1 * math.log(s) + 1)
+    turns = length * plain / (2 * math.pi)
+    ratio = plain / f
+    assert bool((ratio[turns > 64] == 1).all()) and torch.allclose(ratio[turns < 0.5], torch.tensor(s, dtype=torch.float64))
+    assert bool((ratio.diff() >= -1e-12).all()) and float(ratio.min()) >= 1 and float(ratio.max()) <= s + 1e-12
+    _, given = freq(built, 64, scaling={"type": "yarn", "factor": s, "original_max_position": length, "attention_factor": 1.5})
+    assert given == 1.5
+
+
+def test_frequencies_refused(built):
+    for args, kw in (((0,), {}), ((7,), {}), ((64,), {"scaling": {"type": "dynamic", "factor": 2}}), ((64,), {"scaling": {"type": "linear", "factor": 0.5}}),
+                     ((2,), {"scaling": {"type": "ntk", "factor": 2}}), ((64,), {"scaling": {"type": "linear", "factor": float("nan")}})):
+        with pytest.raises(ValueError):
+            freq(built, *args, **kw)
+
+
+def test_c_entries_refuse_before_any_launch(built):
+    lib, at = built._lib.lib(), 64
+    shared = lambda **o: lib.mdb_attn_block_shared(*[{**dict(   # noqa: E731
+        q=at, k=at, v=at, out=at, lse=None, prefix=at, prefix_pages=2, prefix_len=at, table=at, stride=4, pages=4, lens=at, bs=2, block=8, hq=4, hkv=2,
+        num_pages=10, scale=0.1, ws=at, bytes=1 << 40, stream=None), **o}[n] for n in (
+            "q", "k", "v", "out", "lse", "prefix", "prefix_pages", "prefix_len", "table", "stride", "pages", "lens", "bs", "block", "hq", "hkv", "num_pages",
+            "scale", "ws", "bytes", "stream")])
+    assert shared(bs=0) == 0
+    for o, code in (({"q": None}, -1), ({"prefix": None}, -1), ({"prefix_len": None}, -1), ({"hq": 5}, -1), ({"stride": 3}, -1), ({"pages": 0}, -1), ({"bs": -1}, -1),
+                    ({"k": 72}, -2), ({"ws": 72}, -2), ({"hq": 258}, -3), ({"scale": 0.0}, -3), ({"bs": 70000}, -3), ({"scale": float("nan")}, -3),
+                    ({"bytes": 100}, -5), ({"ws": None}, -5)):
+        assert shared(**o) == code, o
+    weights = lambda **o: lib.mdb_key_weights(*[{**dict(   # noqa: E731
+        q=at, k=at, lse=at, table=at, stride=4, pages=4, lens=at, bs=2, block=8, hq=4, hkv=2, num_pages=10, scale=0.1, previous=None, decay=1.0, out=at,
+        cols=100, stream=None), **o}[n] for n in ("q", "k", "lse", "table", "stride", "pages", "lens", "bs", "block", "hq", "hkv", "num_pages", "scale",
+                                                  "previous", "decay", "out", "cols", "stream")])
+    assert weights(bs=0) == 0
+    for o, code in (({"lse": None}, -1), ({"out": None}, -1), ({"cols": 0}, -1), ({"hq": 3}, -1), ({"stride": 1}, -1), ({"q": 72}, -2), ({"hq": 258}, -3), ({"scale": -1.0}, -3),
+                    ({"cols": 1 << 40}, -3)):
+        assert weights(**o) == code, o
+
+    def evict(**o):
+        a = built._lib.KvEvictArgs(bs=1, kv_heads=2, row_bytes=256, budget=10, recent=2, num_pages=4, table_stride=2, table_pages=2, weight_cols=100)
+        for n in ("k_cache", "v_cache", "weights", "seqlens", "seqlens_out", "block_table", "kept"):
+            setattr(a, n, at)
+        for n, v in o.items():
+            setattr(a, n, v)
+        return lib.mdb_kv_evict(ctypes.byref(a), None)
+
+    assert evict(bs=0) == 0 and lib.mdb_kv_evict(None, None) == -1
+    for o, code in (({"recent": 11}, -1), ({"recent": -1}, -1), ({"budget": 0}, -1), ({"kept": None}, -1), ({"weights": None}, -1), ({"out_table": at}, -1),
+                    ({"bs": 2, "table_stride": 1}, -1), ({"row_bytes": 24}, -2), ({"v_cache": 72}, -2), ({"bs": 40000}, -3), ({"row_bytes": 8192}, -3)):
+        assert evict(**o) == code, o
+
+    def rotary(**o):
+        a = built._lib.RotaryEmbedArgs(dtype=0, n=2, heads=2, kv_heads=1, dim=64, rot_dims=64)
+        for n in ("q", "k", "positions", "inv_freq", "q_out", "k_out"):
+            setattr(a, n, at)
+        for n, v in o.items():
+            setattr(a, n, v)
+        return lib.mdb_rotary_embed(ctypes.byref(a), None)
+
+    assert rotary(n=0) == 0 and lib.mdb_rotary_embed(None, None) == -1
+    for o, code in (({"dtype": 2}, -1), ({"rot_dims": 66}, -1), ({"rot_dims": 3}, -1), ({"k": None}, -1), ({"k_out": None}, -1), ({"v": at}, -1), ({"inv_freq": None}, -1),
+                    ({"slots": at}, -1), ({"slots": at, "k_cache": at}, -1), ({"slots": at, "k_cache": at, "num_slots": 5, "v": at}, -1), ({"dim": 2048}, -3),
+                    ({"heads": 5000}, -3)):
+        assert rotary(**o) == code, o
+
+
+def test_workspace_of_the_shared_prefix(built):
+    need = built.ops.shared_prefix_workspace_bytes
+    assert need(0, 32, 16, 8) == 0 and need(4, 32, 16, 5) == 0
+    rows = 4 * 32 * 16
+    assert need(4, 32, 16, 8) >= 2 * rows * 130 * 4
+    assert need(8, 32, 16, 8) > need(4, 32, 16, 8)
+
+
+def test_wrappers_refuse_cpu_tensors(built):
+    x = torch.zeros(2, 1, 64)
+    with pytest.raises(RuntimeError):
+        built.ops.rotary_embed(x, None, torch.arange(2), torch.ones(32, dtype=torch.float64))
+    c = torch.zeros(1, 256, 1, 128, dtype=torch.bfloat16)
+    q, n, t = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        built.ops.block_attn_shared_prefix(q, c, c, None, None, n, t)
+    with pytest.raises(RuntimeError):
+        built.ops.key_weights(q, c, torch.zeros(1, 1, 1), n, t)
+    with pytest.raises(RuntimeError):
+        built.ops.evict_kvcache(c, c, torch.zeros(1, 1, 256), n, t, 10)
