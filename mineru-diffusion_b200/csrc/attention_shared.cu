@@ -13,15 +13,19 @@
 // a unit leaves its sums (max, sum, O: fp32) at the rows' place, a part that goes on with one at its CTA's place (a CTA has one
 // such part at most: its first); info[unit] says how many CTAs follow.
 //
-// Roles: a TMA warp (query tiles, rings of K and V tiles), an MMA warp, four softmax warps per query tile, a row per thread.
-// Tensor memory: S_A (P_A) | S_B (P_B) | O_A | O_B, 128 columns each; with one tile S of even key tiles | - | O | S of odd ones.
-// P goes back into the tensor memory its scores came from, in two halves, of which the first is multiplied while the second is made.
+// Roles: a TMA warp (query tiles, rings of K and V tiles), an MMA warp, two groups of four softmax warps, a row per thread.  Units of
+// two tiles take both groups; units of one take them in turn, each with the query tile, the output columns and the barriers of its
+// group, so that one's start lies under the other's end.
+// Tensor memory: S_0 (P_0) | S_1 (P_1) | O_0 | O_1, 128 columns each.  Of two tiles each has its score columns, of one it takes both in
+// turn, the next scores ahead of P V.  P goes back into the columns its scores came from, in two halves, of which the first is
+// multiplied while the second is made.  The products of one thread run in the order of issue, so scores may follow a P V into
+// the same columns without a wait.
 #include "mdb_common.cuh"
 
 namespace mdb {
 
-// Times in sixteenths of a key tile of one query tile: a key tile of one, of two, start and end of a unit; the least share of a CTA.
-constexpr int kShOneStep = 16, kShTwoStep = 23, kShUnit = 32, kShMinShare = 64;
+// Times: a key tile of one query tile, of two, start and end of a unit; the least share of a CTA.
+constexpr uint32_t kShOneStep = 6, kShTwoStep = 8, kShUnit = 10, kShMinShare = 16;
 
 struct ShPlan {
   static constexpr int kKStages = 3, kVStages = 2;
@@ -45,20 +49,22 @@ struct ShArgs {
   const int32_t* block_table;
   int prefix_pages, table_stride, table_pages, num_pages;
   int bs, block, hq, hkv, group;
-  int tokens;                    // bs * block
-  int box_p, tiles_p, per_p, units_p;      // against the prefix: tokens of a query tile, tiles, tiles per unit, units per key head
-  int box_o, tiles_o, per_o, units_o;      // against a request's own keys
+  int tokens, rows;              // bs * block; rows of a key head: tokens * group
+  int box_p, per_p, units_p;     // against the prefix: tokens of a query tile, tiles per unit, units per key head
+  int box_o, per_o, units_o;     // against a request's own keys
   float scale_log2;
-  float* main_o;                 // [2][tokens * hq][128]: prefix, own
-  float* main_ml;                // [2][tokens * hq][2]: maximum in log2 units, sum
-  float* cont_o;                 // [CTA][256][128]
-  float* cont_ml;
-  int2* info;                    // [hkv * (units_p + bs * units_o)]: CTA of the first part, how many follow
+  // sums of parts lie [channels / 4][rows] of float4: neighbouring rows, neighbouring threads
+  float4* main_o;                // [2: prefix, own][hkv][32][rows]
+  float2* main_ml;               // [2][hkv][rows]: maximum in log2 units, sum
+  float4* cont_o;                // [CTA][32][256]
+  float2* cont_ml;               // [CTA][256]
+  int2* info;                    // [hkv * units_p + bs * hkv * units_o]: CTA of the first part, how many follow
 };
 
+// of a group x: Q, O and P V barriers; S and P barriers by group and score columns
 enum {
-  kShBarQFull = 0, kShBarQEmpty = 1, kShBarKFull = 2, kShBarKEmpty = 5, kShBarVFull = 8, kShBarVEmpty = 10, kShBarSFull = 12 /* 3 */,
-  kShBarPFull = 15 /* 3 x 2 halves */, kShBarPDone = 21, kShBarOFull = 23, kShBarOEmpty = 25, kShBarCount = 27
+  kShBarQFull = 0, kShBarQEmpty = 2, kShBarKFull = 4, kShBarKEmpty = 7, kShBarVFull = 10, kShBarVEmpty = 12, kShBarSFull = 14 /* 2 x + buf */,
+  kShBarPDone = 18, kShBarOFull = 20, kShBarOEmpty = 22, kShBarPFull = 24 /* 2 (2 x + buf) + half */, kShBarCount = 32
 };
 
 __device__ __forceinline__ int sh_prefix(const ShArgs& a) {
@@ -67,68 +73,78 @@ __device__ __forceinline__ int sh_prefix(const ShArgs& a) {
 __device__ __forceinline__ int sh_len(const ShArgs& a, int b) {
   return static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(a.ctx_lens[b]), static_cast<int64_t>(a.table_pages) * kPage)));
 }
-__device__ __forceinline__ int sh_steps(int len) { return len / kAtKeys + (len % kAtKeys != 0); }
-__device__ __forceinline__ int64_t sh_cost(int steps, int per) {
-  return steps == 0 ? 0 : static_cast<int64_t>(steps) * (per == 2 ? kShTwoStep : kShOneStep) + kShUnit;
+__device__ __forceinline__ uint32_t sh_steps(int len) { return (static_cast<uint32_t>(len) + kAtKeys - 1) / kAtKeys; }
+__device__ __forceinline__ uint32_t sh_cost(uint32_t steps, int per) { return steps == 0 ? 0u : steps * (per == 2 ? kShTwoStep : kShOneStep) + kShUnit; }
+// Key tiles of a unit in front of the time x since its start.
+__device__ __forceinline__ uint32_t sh_cut(uint32_t x, uint32_t steps, int per) {
+  if (x <= kShUnit) return 0u;
+  x -= kShUnit;
+  return min(steps, per == 2 ? (x + kShTwoStep / 2) / kShTwoStep : (x + kShOneStep / 2) / kShOneStep);
 }
 
 // A part of a unit.
 struct ShPart {
   int req;                 // -1: the prefix
   int kvh, unit;           // unit: its place in info
-  int tok0, tok1;          // first tokens of tile A and B (of all requests' tokens); tile B is there where `two`
-  bool two;
-  int tok_end;             // the rows end here
-  int box;                 // tokens of a tile
-  int len, k0, k1, steps;  // keys of the unit; key tiles of the part, of the unit
+  int tok0;                // first token of the first tile (of all requests' tokens)
+  bool two;                // there is a second tile
+  int slot;                // group of a unit of one tile
+  int tok_end, box;        // the rows end here; tokens of a tile
+  int len, k0, k1;         // keys of the unit; key tiles of the part
 };
 
 // A CTA's run of the list; every role walks it the same way.
 struct ShWalk {
-  int64_t x0, x1, total, at;     // run, length of the list, start of the unit at the cursor
-  int share;                     // CTAs that have a run
+  uint32_t x0, x1, at;           // run, start of the unit at the cursor
+  uint32_t per, rest, share;     // length of the list = per * share + rest, over so many CTAs
   int plen, len;                 // of the prefix, of the request at the cursor
-  int b, u;                      // cursor: request (-1: prefix), unit among its key heads' units
+  int b, kvh, u;                 // cursor: request (-1: prefix), key head, unit
+  int turn;                      // group of the next unit of one tile
+  __device__ __forceinline__ uint32_t start_of(uint32_t c) const { return per * c + min(c, rest); }
   // by a whole warp
   __device__ __forceinline__ void start(const ShArgs& a) {
     const int lane = threadIdx.x & 31;
+    const uint32_t mine = lane < a.bs ? sh_cost(sh_steps(sh_len(a, lane)), a.per_o) : 0u;
     plen = sh_prefix(a);
-    int64_t own = 0;
-    for (int i = lane; i < a.bs; i += 32) own += sh_cost(sh_steps(sh_len(a, i)), a.per_o);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
-    const int64_t cost_p = sh_cost(sh_steps(plen), a.per_p), all_p = cost_p * a.hkv * a.units_p, per_req = static_cast<int64_t>(a.hkv) * a.units_o;
-    total = all_p + own * per_req;
-    share = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(1), total / kShMinShare)));
-    const int c = static_cast<int>(blockIdx.x);
+    uint32_t own = mine;
+    for (int i = lane + 32; i < a.bs; i += 32) own += sh_cost(sh_steps(sh_len(a, i)), a.per_o);
+    own = __reduce_add_sync(0xffffffffu, own);
+    const uint32_t cost_p = sh_cost(sh_steps(plen), a.per_p), per_req = static_cast<uint32_t>(a.hkv * a.units_o);
+    const uint32_t all_p = cost_p * static_cast<uint32_t>(a.hkv * a.units_p), total = all_p + own * per_req;
+    share = min(gridDim.x, max(1u, total / kShMinShare));
+    per = total / share;
+    rest = total - per * share;
     x0 = x1 = at = 0;
-    b = -1; u = 0; len = 0;
-    if (c >= share) return;
-    x0 = total * c / share;
-    x1 = total * (c + 1) / share;
+    b = -1; kvh = 0; u = 0; len = 0; turn = 0;
+    if (blockIdx.x >= share) return;
+    x0 = start_of(blockIdx.x);
+    x1 = start_of(blockIdx.x + 1);
     if (x0 < all_p) {
-      u = static_cast<int>(x0 / cost_p);
-      at = u * cost_p;
+      const uint32_t i = x0 / cost_p;
+      at = i * cost_p;
+      kvh = static_cast<int>(i) / a.units_p;
+      u = static_cast<int>(i) - kvh * a.units_p;
       return;
     }
     at = all_p;
     for (int b0 = 0; b0 < a.bs; b0 += 32) {
-      const int i = b0 + lane;
-      const int64_t mine = i < a.bs ? sh_cost(sh_steps(sh_len(a, i)), a.per_o) * per_req : 0;
-      int64_t upto = mine;
+      const uint32_t c = b0 == 0 ? mine : b0 + lane < a.bs ? sh_cost(sh_steps(sh_len(a, b0 + lane)), a.per_o) : 0u;
+      uint32_t upto = c * per_req;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += up;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, x0 < at + upto);
       if (hit) {
         const int l = __ffs(hit) - 1;
         b = b0 + l;
-        at += __shfl_sync(0xffffffffu, upto - mine, l);
-        const int64_t each = __shfl_sync(0xffffffffu, mine, l) / per_req;
-        u = static_cast<int>((x0 - at) / each);
-        at += u * each;
+        const uint32_t each = __shfl_sync(0xffffffffu, c, l);
+        at += __shfl_sync(0xffffffffu, upto, l) - each * per_req;
+        const uint32_t i = (x0 - at) / each;
+        at += i * each;
+        kvh = static_cast<int>(i) / a.units_o;
+        u = static_cast<int>(i) - kvh * a.units_o;
         len = sh_len(a, b);
         return;
       }
@@ -139,41 +155,44 @@ struct ShWalk {
   __device__ __forceinline__ bool next(const ShArgs& a, ShPart& p) {
     while (at < x1) {
       const bool prefix = b < 0;
-      const int units = prefix ? a.units_p : a.units_o, per = prefix ? a.per_p : a.per_o;
-      const int n = prefix ? plen : len, steps = sh_steps(n);
-      if (steps == 0 || u == a.hkv * units) {              // behind the units of the prefix or of a request
-        ++b;
-        u = 0;
-        if (b >= a.bs) return false;
+      const int units = prefix ? a.units_p : a.units_o, tiles = prefix ? a.per_p : a.per_o, n = prefix ? plen : len;
+      const uint32_t steps = sh_steps(n);
+      if (steps == 0 || kvh == a.hkv) {                    // behind the units of the prefix or of a request
+        if (++b >= a.bs) return false;
+        kvh = 0; u = 0;
         len = sh_len(a, b);
         continue;
       }
-      const int64_t cost = sh_cost(steps, per);
-      p.k0 = x0 <= at ? 0 : static_cast<int>((x0 - at) * steps / cost);
-      p.k1 = x1 >= at + cost ? steps : static_cast<int>((x1 - at) * steps / cost);
+      const uint32_t cost = sh_cost(steps, tiles);
+      p.k0 = x0 <= at ? 0 : static_cast<int>(sh_cut(x0 - at, steps, tiles));
+      p.k1 = static_cast<int>(x1 >= at + cost ? steps : sh_cut(x1 - at, steps, tiles));
       p.req = b;
-      p.kvh = u / units;
-      p.unit = prefix ? u : a.hkv * (a.units_p + b * a.units_o) + u;
+      p.kvh = kvh;
+      p.unit = (prefix ? 0 : a.hkv * (a.units_p + b * a.units_o)) + kvh * units + u;
       p.box = prefix ? a.box_p : a.box_o;
-      const int first = (u % units) * per;
-      p.tok0 = (prefix ? 0 : b * a.block) + first * p.box;
-      p.tok1 = p.tok0 + p.box;
+      p.tok0 = (prefix ? 0 : b * a.block) + u * tiles * p.box;
       p.tok_end = prefix ? a.tokens : (b + 1) * a.block;
-      p.two = per == 2 && p.tok1 < p.tok_end;
-      p.len = n; p.steps = steps;
+      p.two = tiles == 2 && p.tok0 + p.box < p.tok_end;
+      p.len = n;
       at += cost;
-      ++u;
-      if (p.k1 > p.k0) return true;
+      if (++u == units) { u = 0; ++kvh; }
+      if (p.k1 > p.k0) {
+        p.slot = turn;
+        if (!p.two) turn ^= 1;
+        return true;
+      }
     }
     return false;
   }
   // how many CTAs behind this one have a part of the unit that `next` gave last
   __device__ __forceinline__ int followers(const ShArgs& a, const ShPart& p) const {
-    const int64_t cost = sh_cost(p.steps, p.req < 0 ? a.per_p : a.per_o), s = at - cost;
+    const uint32_t steps = sh_steps(p.len);
+    const int tiles = p.req < 0 ? a.per_p : a.per_o;
+    const uint32_t s = at - sh_cost(steps, tiles);
     int n = 0;
-    for (int c = static_cast<int>(blockIdx.x) + 1; c < share; ++c, ++n) {
-      const int64_t x = total * c / share;
-      if (x >= at || (x - s) * p.steps / cost >= p.steps) break;
+    for (uint32_t c = blockIdx.x + 1; c < share; ++c, ++n) {
+      const uint32_t x = start_of(c);
+      if (x >= at || sh_cut(x - s, steps, tiles) >= steps) break;
     }
     return n;
   }
@@ -184,7 +203,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ uint32_t sh_score_col(int buf) { return buf == 2 ? 384u : 128u * buf; }
 
 __global__ void __launch_bounds__(ShPlan::kThreads, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_constant__ CUtensorMap map_qo, const __grid_constant__ CUtensorMap map_k,
@@ -200,8 +218,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kShBarCount; ++s) mbar_init(bar(s), (s >= kShBarPFull && s < kShBarPFull + 6) || s >= kShBarOEmpty ? 4 : 1);
+  if (warp == 0) {
+    mbar_init(bar(lane), lane >= kShBarOEmpty ? 4 : 1);      // (those of the softmax warps are the last ones)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -224,8 +242,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
       // ------------------------------------------------------------------ producer
       if (lane == 0) {
         AtRing kr, vr;
-        uint32_t q_phase = 0;
-        uint32_t pend_k = 0, pend_v = 0, pend_q = 0;          // stages with a copy in flight, and the parity it completes
+        uint32_t q_phase = 0, pend_k = 0, pend_v = 0, pend_q = 0;     // stages with a copy in flight, and the parity it completes
         uint32_t par_k = 0, par_v = 0, par_q = 0;
         bool ok = true;
         auto load_tile = [&](const CUtensorMap* map, uint32_t tiles0, int full0, int empty0, int stages, AtRing& r, uint32_t& pend, uint32_t& par,
@@ -242,24 +259,23 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
         };
         if (blockIdx.x == 0 && a.prefix_len != nullptr && *a.prefix_len > walk.plen) report_status(MDB_STATUS_BAD_PAGE);
         while (ok && walk.next(a, w)) {
-          if (w.req >= 0 && w.k0 == 0 && a.ctx_lens[w.req] > w.len) report_status(MDB_STATUS_BAD_PAGE);
-          if (!mbar_wait(bar(kShBarQEmpty), q_phase ^ 1)) { ok = false; break; }
-          const CUtensorMap* map_q = w.req < 0 ? &map_qp : &map_qo;
-          mbar_arrive_expect_tx(bar(kShBarQFull), static_cast<uint32_t>(w.box * a.group) * 256u * (w.two ? 2u : 1u));
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (x == 1 && !w.two) break;
-            const uint32_t dst = base + x * P::kQBytes;
-            const int tok = x == 0 ? w.tok0 : w.tok1;
-            tma_load_3d(dst, map_q, 0, w.kvh * a.group, tok, bar(kShBarQFull));
-            tma_load_3d(dst + 128 * 128, map_q, 64, w.kvh * a.group, tok, bar(kShBarQFull));
-          }
-          pend_q = 1u;
-          par_q = q_phase;
-          q_phase ^= 1;
           const int32_t* table = w.req < 0 ? a.prefix_table : a.block_table + static_cast<int64_t>(w.req) * a.table_stride;
+          int page = table[w.k0 * kAtKeys / kPage];
+          if (w.req >= 0 && w.k0 == 0 && a.ctx_lens[w.req] > w.len) report_status(MDB_STATUS_BAD_PAGE);
+          const CUtensorMap* map_q = w.req < 0 ? &map_qp : &map_qo;
+          for (int x = w.two ? 0 : w.slot; x <= (w.two ? 1 : w.slot); ++x) {
+            if (!mbar_wait(bar(kShBarQEmpty + x), (q_phase >> x & 1) ^ 1)) { ok = false; break; }
+            const uint32_t dst = base + x * P::kQBytes, full = bar(kShBarQFull + x);
+            const int tok = w.tok0 + (w.two ? x * w.box : 0);
+            mbar_arrive_expect_tx(full, static_cast<uint32_t>(w.box * a.group) * 256u);
+            tma_load_3d(dst, map_q, 0, w.kvh * a.group, tok, full);
+            tma_load_3d(dst + 128 * 128, map_q, 64, w.kvh * a.group, tok, full);
+            pend_q |= 1u << x;
+            par_q = (par_q & ~(1u << x)) | (q_phase & 1u << x);
+            q_phase ^= 1u << x;
+          }
           for (int j = w.k0; j < w.k1 && ok; ++j) {
-            int page = table[j * kAtKeys / kPage];
+            if (j > w.k0 && j * kAtKeys % kPage == 0) page = table[j * kAtKeys / kPage];
             if (page < 0 || page >= a.num_pages) {
               report_status(MDB_STATUS_BAD_PAGE);
               page = 0;
@@ -274,7 +290,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
           // let the copies already issued land before the CTA gives its shared memory back
           for (int s = 0; s < P::kKStages; ++s) if (pend_k >> s & 1) mbar_wait(bar(kShBarKFull + s), par_k >> s & 1);
           for (int s = 0; s < P::kVStages; ++s) if (pend_v >> s & 1) mbar_wait(bar(kShBarVFull + s), par_v >> s & 1);
-          if (pend_q) mbar_wait(bar(kShBarQFull), par_q);
+          for (int s = 0; s < 2; ++s) if (pend_q >> s & 1) mbar_wait(bar(kShBarQFull + s), par_q >> s & 1);
         }
       }
     } else if (warp == kMmaWarp) {
@@ -283,72 +299,113 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
       const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kAtKeys >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
       const uint32_t idesc_o = idesc_s | (1u << 16);
       AtRing kr, vr;
-      uint32_t p_phase = 0 /* bit per score buffer */, o_phase[2] = {0, 0}, q_phase = 0;
-      bool ok = true;
-      while (ok && walk.next(a, w)) {
-        const bool alone = !w.two;
-        if (!mbar_wait_w(bar(kShBarQFull), q_phase)) { ok = false; break; }
-        q_phase ^= 1;
-        auto issue_s = [&](int x, int buf) {           // scores of tile x with the K tile at the ring's position
-          const uint32_t q_tile = base + x * P::kQBytes, k_tile = base + P::kOffK + kr.stage * kAtTileBytes;
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            umma_bf16_x4_w(tmem_base + sh_score_col(buf), umma_desc_sw128(q_tile + c * (128 * 128)), 2, umma_desc_sw128(k_tile + c * kAtHalfBytes), 2, idesc_s, c);
-          umma_commit_w(bar(kShBarSFull + buf));
-        };
-        auto release_k = [&](int j) {
-          umma_commit_w(bar(kShBarKEmpty + kr.stage));
-          kr.advance(P::kKStages);
-          if (j == w.k1 - 1) umma_commit_w(bar(kShBarQEmpty));
-        };
-        if (!mbar_wait_w(bar(kShBarKFull + kr.stage), kr.phase)) { ok = false; break; }
+      uint32_t p_phase = 0 /* bit 2 x + buf */, o_phase = 0, q_phase = 0 /* bit x */;
+      int buf = 0;                         // score columns of the next tile of a unit of one
+      bool ok = true, have = walk.next(a, w), ahead = false;
+      auto wait_q = [&](int x) {
+        const bool r = mbar_wait_w(bar(kShBarQFull + x), q_phase >> x & 1);
+        q_phase ^= 1u << x;
+        return r;
+      };
+      auto wait_k = [&]() {
+        const bool r = mbar_wait_w(bar(kShBarKFull + kr.stage), kr.phase);
         tc_fence_after();
-        issue_s(0, 0);
-        if (w.two) issue_s(1, 1);
-        release_k(w.k0);
-        for (int j = w.k0; j < w.k1 && ok; ++j) {
-          const bool more = j + 1 < w.k1;
-          const int odd = (j - w.k0) & 1;
-          bool k_there = false;
-          if (alone && more) {
-            // the other buffer held the last key tile, whose P V has been issued; or an output of tile B that must have been read out
-            if (j == w.k0 && !mbar_wait_w(bar(kShBarOEmpty + 1), o_phase[1] ^ 1)) { ok = false; break; }
-            if (!mbar_wait_w(bar(kShBarKFull + kr.stage), kr.phase)) { ok = false; break; }
-            tc_fence_after();
-            issue_s(0, odd ? 0 : 2);
-            release_k(j + 1);
-          }
-          if (!mbar_wait_w(bar(kShBarVFull + vr.stage), vr.phase)) { ok = false; break; }
+        return r;
+      };
+      auto issue_s = [&](int x, int to) {  // scores of the query tile of group x with the K tile at the ring's position
+        const uint32_t q_tile = base + x * P::kQBytes, k_tile = base + P::kOffK + kr.stage * kAtTileBytes;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (x == 1 && alone) break;
-            const int buf = alone && odd ? 2 : x;
-            if (j == w.k0) {
-              // the previous unit's accumulator must have been read out
-              if (!mbar_wait_w(bar(kShBarOEmpty + x), o_phase[x] ^ 1)) { ok = false; break; }
-              o_phase[x] ^= 1;
+        for (int c = 0; c < 2; ++c)
+          umma_bf16_x4_w(tmem_base + 128 * to, umma_desc_sw128(q_tile + c * (128 * 128)), 2, umma_desc_sw128(k_tile + c * kAtHalfBytes), 2, idesc_s, c);
+        umma_commit_w(bar(kShBarSFull + 2 * x + to));
+      };
+      auto release_k = [&]() {
+        umma_commit_w(bar(kShBarKEmpty + kr.stage));
+        kr.advance(P::kKStages);
+      };
+      // O of group x (+)= P of `from` times the V tile at the ring's position
+      auto issue_o = [&](int x, int from, bool first, bool last) {
+        if (first) {
+          // the output of the group's unit before must have been read out
+          if (!mbar_wait_w(bar(kShBarOEmpty + x), (o_phase >> x & 1) ^ 1)) return false;
+          o_phase ^= 1u << x;
+        }
+        const int i = 2 * x + from;
+        const uint32_t v_tile = base + P::kOffV + vr.stage * kAtTileBytes, p = tmem_base + 128 * from, o = tmem_base + 256 + x * 128;
+        if (!mbar_wait_w(bar(kShBarPFull + 2 * i), p_phase >> i & 1)) return false;
+        tc_fence_after();
+        umma_bf16_ts_x4_w(o, p, umma_desc_sw128_mn(v_tile), 128, idesc_o, first ? 0u : 1u);
+        if (!mbar_wait_w(bar(kShBarPFull + 2 * i + 1), p_phase >> i & 1)) return false;
+        p_phase ^= 1u << i;
+        tc_fence_after();
+        umma_bf16_ts_x4_w(o, p + 32, umma_desc_sw128_mn(v_tile + 4 * 2048), 128, idesc_o, 1u);
+        umma_commit_w(bar(kShBarPDone + x));
+        if (last) umma_commit_w(bar(kShBarOFull + x));
+        return true;
+      };
+      while (ok && have) {
+        if (w.two) {
+          ok = wait_q(0) && wait_q(1) && wait_k();
+          if (!ok) break;
+          issue_s(0, 0);
+          issue_s(1, 1);
+          release_k();
+          if (w.k1 == w.k0 + 1) { umma_commit_w(bar(kShBarQEmpty)); umma_commit_w(bar(kShBarQEmpty + 1)); }
+          for (int j = w.k0; j < w.k1; ++j) {
+            const bool first = j == w.k0, last = j + 1 == w.k1;
+            ok = mbar_wait_w(bar(kShBarVFull + vr.stage), vr.phase) && issue_o(0, 0, first, last);
+            if (!ok) break;
+            if (!last) {
+              ok = wait_k();
+              if (!ok) break;
+              issue_s(0, 0);
             }
-            const uint32_t v_tile = base + P::kOffV + vr.stage * kAtTileBytes, p = tmem_base + sh_score_col(buf), o = tmem_base + 256 + x * 128;
-            if (!mbar_wait_w(bar(kShBarPFull + 2 * buf), p_phase >> buf & 1)) { ok = false; break; }
-            tc_fence_after();
-            umma_bf16_ts_x4_w(o, p, umma_desc_sw128_mn(v_tile), 128, idesc_o, j > w.k0 ? 1u : 0u);
-            if (!mbar_wait_w(bar(kShBarPFull + 2 * buf + 1), p_phase >> buf & 1)) { ok = false; break; }
-            p_phase ^= 1u << buf;
-            tc_fence_after();
-            umma_bf16_ts_x4_w(o, p + 32, umma_desc_sw128_mn(v_tile + 4 * 2048), 128, idesc_o, 1u);
-            umma_commit_w(bar(kShBarPDone + x));
-            if (!more) umma_commit_w(bar(kShBarOFull + x));
-            if (!alone && more) {
-              if (!k_there && !mbar_wait_w(bar(kShBarKFull + kr.stage), kr.phase)) { ok = false; break; }
-              k_there = true;
-              tc_fence_after();
-              issue_s(x, x);
+            ok = issue_o(1, 1, first, last);
+            if (!ok) break;
+            umma_commit_w(bar(kShBarVEmpty + vr.stage));
+            vr.advance(P::kVStages);
+            if (!last) {
+              issue_s(1, 1);
+              release_k();
+              if (j + 2 == w.k1) { umma_commit_w(bar(kShBarQEmpty)); umma_commit_w(bar(kShBarQEmpty + 1)); }
             }
           }
-          if (!ok) break;
-          umma_commit_w(bar(kShBarVEmpty + vr.stage));
-          vr.advance(P::kVStages);
-          if (!alone && more) release_k(j + 1);
+          have = ok && walk.next(a, w);
+        } else {
+          const int x = w.slot, k0 = w.k0, k1 = w.k1;
+          if (!ahead) {
+            ok = wait_q(x) && wait_k();
+            if (!ok) break;
+            issue_s(x, buf);
+            release_k();
+            if (k1 == k0 + 1) umma_commit_w(bar(kShBarQEmpty + x));
+          }
+          ahead = false;
+          for (int j = k0; j < k1; ++j) {
+            // the next scores first: of this unit, or of the next one where that is of one tile too
+            if (j + 1 < k1) {
+              ok = wait_k();
+              if (!ok) break;
+              issue_s(x, buf ^ 1);
+              release_k();
+              if (j + 2 == k1) umma_commit_w(bar(kShBarQEmpty + x));
+            } else {
+              have = walk.next(a, w);
+              if (have && !w.two) {
+                ok = wait_q(w.slot) && wait_k();
+                if (!ok) break;
+                issue_s(w.slot, buf ^ 1);
+                release_k();
+                if (w.k1 == w.k0 + 1) umma_commit_w(bar(kShBarQEmpty + w.slot));
+                ahead = true;
+              }
+            }
+            ok = mbar_wait_w(bar(kShBarVFull + vr.stage), vr.phase) && issue_o(x, buf, j == k0, j + 1 == k1);
+            if (!ok) break;
+            umma_commit_w(bar(kShBarVEmpty + vr.stage));
+            vr.advance(P::kVStages);
+            buf ^= 1;
+          }
         }
       }
       if (!ok && lane == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
@@ -356,150 +413,162 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
   } else {
     // ------------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kSoftmaxRegs));
-    const int x = warp >> 2;                               // tile A or B
+    const int x = warp >> 2;                               // group
     const int row = threadIdx.x & 127;                     // query row of the tile, and its tensor-memory lane
-    const int tok_local = row / a.group, head_in_group = row % a.group;
+    const int tok_local = row / a.group;
     const uint32_t lane_field = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t o_addr = tmem_base + 256 + x * 128 + lane_field;
     const f32x2 scale = pack2(a.scale_log2, a.scale_log2);
     AtRing vr;                          // V ring position of the part's first key tile
-    uint32_t s_phase = 0 /* bit per buffer */, o_phase = 0, done_phase = 0;      // done: of the last P V
+    int buf0 = 0;                       // score columns of its first tile, in a unit of one
+    uint32_t s_phase = 0 /* bit per score columns */, o_phase = 0, done_phase = 0;      // done: of the last P V
     bool ok = true;
     while (ok && walk.next(a, w)) {
       const int tiles = w.k1 - w.k0;
-      if (x == 0 && threadIdx.x == 0 && w.k0 == 0) a.info[w.unit] = make_int2(static_cast<int>(blockIdx.x), walk.followers(a, w));
-      auto skip_v = [&]() { vr.phase ^= (vr.stage + tiles) / P::kVStages & 1; vr.stage = (vr.stage + tiles) % P::kVStages; };
-      if (x == 1 && !w.two) {
-        skip_v();
-        continue;
-      }
-      const int tok = (x == 0 ? w.tok0 : w.tok1) + tok_local;
-      const bool row_valid = tok_local < w.box && tok < w.tok_end;
-      const bool warp_valid = __any_sync(0xffffffffu, row_valid);
-      float m_ref = -INFINITY, l = 0.f;
-      for (int j = w.k0; j < w.k1; ++j) {
-        const int odd = (j - w.k0) & 1, buf = !w.two && odd ? 2 : x;
-        const uint32_t s_addr = tmem_base + sh_score_col(buf) + lane_field;
-        ok = mbar_wait(bar(kShBarSFull + buf), s_phase >> buf & 1);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        s_phase ^= 1u << buf;
-        tc_fence_after();
-        const int nv = w.len - j * kAtKeys;               // keys of this tile: [0, nv)
-        if (nv < kAtKeys) {
-          // stale rows behind the last key must not reach O through 0 * (Inf or NaN): clear their values
-          const int v_at = vr.stage + (j - w.k0), v_stage = v_at % P::kVStages;
-          ok = mbar_wait(bar(kShBarVFull + v_stage), vr.phase ^ (v_at / P::kVStages & 1));
+      const bool mine = w.two || w.slot == x;
+      if (row == 0 && w.k0 == 0 && (w.two ? x == 0 : mine)) a.info[w.unit] = make_int2(static_cast<int>(blockIdx.x), walk.followers(a, w));
+      if (mine) {
+        const int tok = w.tok0 + (w.two ? x * w.box : 0) + tok_local;
+        const bool row_valid = tok_local < w.box && tok < w.tok_end;
+        const bool warp_valid = __any_sync(0xffffffffu, row_valid);
+        float m_ref = -INFINITY, l = 0.f;
+        for (int j = w.k0; j < w.k1; ++j) {
+          const int buf = w.two ? x : (buf0 + j - w.k0) & 1;
+          const uint32_t s_addr = tmem_base + 128 * buf + lane_field;
+          ok = mbar_wait(bar(kShBarSFull + 2 * x + buf), s_phase >> buf & 1);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const int r = nv + row;
-          if (r < kAtKeys) {
-            const uint32_t v_row = base + P::kOffV + v_stage * kAtTileBytes + r * 128;
-#pragma unroll
-            for (int c = 0; c < 16; ++c)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_row + (c >> 3) * kAtHalfBytes + (c & 7) * 16), "r"(0u) : "memory");
-          }
-          fence_async_smem();
-        }
-        if (warp_valid) {
-          float s[kAtKeys];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
-          tmem_ld_wait();
+          s_phase ^= 1u << buf;
+          tc_fence_after();
+          const int nv = w.len - j * kAtKeys;               // keys of this tile: [0, nv)
           if (nv < kAtKeys) {
+            // stale rows behind the last key must not reach O through 0 * (Inf or NaN): clear their values
+            const int v_at = vr.stage + (j - w.k0), v_stage = v_at % P::kVStages;
+            ok = mbar_wait(bar(kShBarVFull + v_stage), vr.phase ^ (v_at / P::kVStages & 1));
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const int r = nv + row;
+            if (r < kAtKeys) {
+              const uint32_t v_row = base + P::kOffV + v_stage * kAtTileBytes + r * 128;
 #pragma unroll
-            for (int c = 0; c < kAtKeys; ++c) if (c >= nv) s[c] = -INFINITY;   // also replaces NaN from stale rows
+              for (int c = 0; c < 16; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_row + (c >> 3) * kAtHalfBytes + (c & 7) * 16), "r"(0u) : "memory");
+            }
+            fence_async_smem();
           }
-          float mxv[4];
+          const uint32_t p_full = bar(kShBarPFull + 2 * (2 * x + buf));
+          if (warp_valid) {
+            float s[kAtKeys];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mxv[k] = fmaxf(s[k], s[4 + k]);
+            for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
+            tmem_ld_wait();
+            if (nv < kAtKeys) {
 #pragma unroll
-          for (int c = 8; c < kAtKeys; c += 8)
+              for (int c = 0; c < kAtKeys; ++c) if (c >= nv) s[c] = -INFINITY;   // also replaces NaN from stale rows
+            }
+            float mxv[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mxv[k] = max3(mxv[k], s[c + k], s[c + 4 + k]);
-          float mx = fmaxf(fmaxf(mxv[0], mxv[1]), fmaxf(mxv[2], mxv[3]));
-          if (!row_valid) mx = 0.f;                             // rows that are not there hold whatever the tile held
-          const float m_tile = mx * a.scale_log2;
-          const bool grow = m_tile > m_ref + kAtRescaleStep || (m_ref == -INFINITY && m_tile != -INFINITY);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float m_new = fmaxf(m_ref, m_tile);
-            const float f = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
-            l *= f;
-            if (j > w.k0) {
-              // O is quiet once the last key tile's P V has completed (the one before completed before these scores)
-              ok = mbar_wait(bar(kShBarPDone + x), done_phase ^ 1);
-              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-              tc_fence_after();
+            for (int k = 0; k < 4; ++k) mxv[k] = fmaxf(s[k], s[4 + k]);
+#pragma unroll
+            for (int c = 8; c < kAtKeys; c += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mxv[k] = max3(mxv[k], s[c + k], s[c + 4 + k]);
+            float mx = fmaxf(fmaxf(mxv[0], mxv[1]), fmaxf(mxv[2], mxv[3]));
+            if (!row_valid) mx = 0.f;                             // rows that are not there hold whatever the tile held
+            const float m_tile = mx * a.scale_log2;
+            const bool grow = m_tile > m_ref + kAtRescaleStep || (m_ref == -INFINITY && m_tile != -INFINITY);
+            if (__any_sync(0xffffffffu, grow)) {
+              const float m_new = fmaxf(m_ref, m_tile);
+              const float f = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
+              l *= f;
+              if (j > w.k0) {
+                // O is quiet once the last key tile's P V has completed (the one before completed before these scores)
+                ok = mbar_wait(bar(kShBarPDone + x), done_phase ^ 1);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                float o[32];
-                tmem_ld32(o_addr + 32 * c, o);
-                tmem_ld_wait();
+                for (int c = 0; c < 4; ++c) {
+                  float o[32];
+                  tmem_ld32(o_addr + 32 * c, o);
+                  tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= f;
-                tmem_st32(o_addr + 32 * c, o);
+                  for (int e = 0; e < 32; ++e) o[e] *= f;
+                  tmem_st32(o_addr + 32 * c, o);
+                }
               }
+              m_ref = m_new;
             }
-            m_ref = m_new;
-          }
-          // P = 2^(s * scale - m_ref) rounded to bf16 (the left operand of P V has the type of V); a masked key gives 2^-inf = 0
-          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;   // nothing seen yet: every s is -inf, P = 0
-          const f32x2 minus = pack2(-m_use, -m_use);
-          f32x2 lv[4] = {0ull, 0ull, 0ull, 0ull};
+            // P = 2^(s * scale - m_ref) rounded to bf16 (the left operand of P V has the type of V); a masked key gives 2^-inf = 0
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;   // nothing seen yet: every s is -inf, P = 0
+            const f32x2 minus = pack2(-m_use, -m_use);
+            f32x2 lv[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float pk[32];                                         // 64 keys, two per word
+            for (int h = 0; h < 2; ++h) {
+              float pk[32];                                         // 64 keys, two per word
 #pragma unroll
-            for (int c = 0; c < 64; c += 8) {
-              float2 y[4];
+              for (int c = 0; c < 64; c += 8) {
+                float2 y[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                y[k] = unpack2(fma2(pack2(s[64 * h + c + 2 * k], s[64 * h + c + 2 * k + 1]), scale, minus));
-                y[k].x = ex2_approx(y[k].x);
-                y[k].y = ex2_approx(y[k].y);
-                lv[k] = add2(lv[k], pack2(y[k].x, y[k].y));
-                pk[(c >> 1) + k] = __uint_as_float(pack_bf16x2(y[k].x, y[k].y));
+                for (int k = 0; k < 4; ++k) {
+                  y[k] = unpack2(fma2(pack2(s[64 * h + c + 2 * k], s[64 * h + c + 2 * k + 1]), scale, minus));
+                  y[k].x = ex2_approx(y[k].x);
+                  y[k].y = ex2_approx(y[k].y);
+                  lv[k] = add2(lv[k], pack2(y[k].x, y[k].y));
+                  pk[(c >> 1) + k] = __uint_as_float(pack_bf16x2(y[k].x, y[k].y));
+                }
               }
+              tmem_st32(s_addr + 32 * h, pk);
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_full + 8 * h);
             }
-            tmem_st32(s_addr + 32 * h, pk);
-            tmem_st_wait();
-            tc_fence_before();
+            const float2 ls = unpack2(add2(add2(lv[0], lv[1]), add2(lv[2], lv[3])));
+            l += ls.x + ls.y;
+          } else {
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kShBarPFull + 2 * buf + h));
+            if (lane == 0) { mbar_arrive(p_full); mbar_arrive(p_full + 8); }
           }
-          const float2 ls = unpack2(add2(add2(lv[0], lv[1]), add2(lv[2], lv[3])));
-          l += ls.x + ls.y;
-        } else {
-          __syncwarp();
-          if (lane == 0) { mbar_arrive(bar(kShBarPFull + 2 * buf)); mbar_arrive(bar(kShBarPFull + 2 * buf + 1)); }
+          done_phase ^= 1;
         }
-        done_phase ^= 1;
-      }
-      if (!ok) break;
-      skip_v();
-      // ------------------------------------------------------------- sums of the tile
-      ok = mbar_wait(bar(kShBarOFull + x), o_phase);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      o_phase ^= 1;
-      tc_fence_after();
-      if (warp_valid) {
-        const int64_t rows = static_cast<int64_t>(a.tokens) * a.hq;
-        const int64_t at = w.k0 > 0 ? static_cast<int64_t>(blockIdx.x) * 256 + x * 128 + row
-                                    : (w.req < 0 ? 0 : rows) + static_cast<int64_t>(tok) * a.hq + w.kvh * a.group + head_in_group;
-        float4* po = reinterpret_cast<float4*>((w.k0 > 0 ? a.cont_o : a.main_o) + at * kHeadDim);
+        if (!ok) break;
+        // ------------------------------------------------------------- sums of the tile
+        ok = mbar_wait(bar(kShBarOFull + x), o_phase);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        o_phase ^= 1;
+        tc_fence_after();
+        if (warp_valid) {
+          float4* po;
+          float2* pm;
+          int64_t stride;
+          if (w.k0 > 0) {
+            const int at = (w.two ? x * 128 : 0) + row;
+            stride = 256;
+            po = a.cont_o + static_cast<int64_t>(blockIdx.x) * 32 * 256 + at;
+            pm = a.cont_ml + static_cast<int64_t>(blockIdx.x) * 256 + at;
+          } else {
+            const int64_t head = (w.req < 0 ? 0 : a.hkv) + w.kvh, at = static_cast<int64_t>(tok) * a.group + row % a.group;
+            stride = a.rows;
+            po = a.main_o + head * 32 * stride + at;
+            pm = a.main_ml + head * stride + at;
+          }
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          tmem_ld32(o_addr + 32 * c, o);
-          tmem_ld_wait();
-          if (row_valid) {
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            tmem_ld32(o_addr + 32 * c, o);
+            tmem_ld_wait();
+            if (row_valid) {
 #pragma unroll
-            for (int q4 = 0; q4 < 8; ++q4) po[8 * c + q4] = make_float4(o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]);
+              for (int q4 = 0; q4 < 8; ++q4) po[(8 * c + q4) * stride] = make_float4(o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]);
+            }
           }
+          if (row_valid) *pm = make_float2(m_ref, l);
         }
-        if (row_valid) *reinterpret_cast<float2*>((w.k0 > 0 ? a.cont_ml : a.main_ml) + at * 2) = make_float2(m_ref, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kShBarOEmpty + x));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kShBarOEmpty + x));
+      vr.phase ^= (vr.stage + tiles) / P::kVStages & 1;
+      vr.stage = (vr.stage + tiles) % P::kVStages;
+      if (!w.two) buf0 = (buf0 + tiles) & 1;
     }
     if (!ok && lane == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
   }
@@ -512,56 +581,86 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
   }
 }
 
-// Joins a row's parts: prefix, CTAs that went on with it, own keys, CTAs that went on with them, in this order; a warp per row.
+// Joins the parts of 32 rows of a key head: prefix, CTAs that went on with it, own keys, CTAs that went on with them, in this order.  A
+// lane per row, 16 channels per warp.
 __global__ void __launch_bounds__(256) attn_shared_merge(const ShArgs a) {
   pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) * 4, kvh = blockIdx.y;
+  const int at = static_cast<int>(blockIdx.x) * 32 + lane;
+  const int tok = at / a.group, g = at - tok * a.group, b = tok / a.block, t = tok - b * a.block;
   pdl_wait();
-  const int64_t rows = static_cast<int64_t>(a.tokens) * a.hq, r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  const int tok = static_cast<int>(r / a.hq), head = static_cast<int>(r % a.hq), kvh = head / a.group, g = head % a.group;
-  const int b = tok / a.block, t = tok % a.block;
+  if (at >= a.rows) return;
   float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto join = [&](const float* o, const float* ml, int64_t at) {
-    const float2 p = *reinterpret_cast<const float2*>(ml + at * 2);
-    const float4 v = *reinterpret_cast<const float4*>(o + at * kHeadDim + lane * 4);
+  float4 acc[4] = {};
+  auto join = [&](const float2 p, const float4 (&v)[4]) {
     if (p.x == -INFINITY) return;                          // (scores that are all -inf)
     const float m_new = fmaxf(m, p.x), f = ex2_approx(m - m_new), w = ex2_approx(p.x - m_new);
     m = m_new;
     l = l * f + p.y * w;
-    acc.x = acc.x * f + v.x * w; acc.y = acc.y * f + v.y * w; acc.z = acc.z * f + v.z * w; acc.w = acc.w * f + v.w * w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc[i].x = acc[i].x * f + v[i].x * w; acc[i].y = acc[i].y * f + v[i].y * w;
+      acc[i].z = acc[i].z * f + v[i].z * w; acc[i].w = acc[i].w * f + v[i].w * w;
+    }
   };
+  // what may be there is asked for before it is known whether it is
+  float2 first_ml[2];
+  float4 first[2][4];
+  int2 more[2];
+  int place[2], len[2];
 #pragma unroll
   for (int own = 0; own < 2; ++own) {
-    const int len = own ? sh_len(a, b) : sh_prefix(a);
-    if (len == 0) continue;
-    const int box = own ? a.box_o : a.box_p, per = own ? a.per_o : a.per_p, units = own ? a.units_o : a.units_p;
-    const int at = own ? t : tok, tile = at / box;
-    const int unit = (own ? a.hkv * (a.units_p + b * a.units_o) : 0) + kvh * units + tile / per;
-    const int2 more = a.info[unit];
-    join(a.main_o, a.main_ml, (own ? rows : 0) + r);
-    const int64_t place = static_cast<int64_t>(tile % per) * 128 + (at % box) * a.group + g;
-    for (int c = 1; c <= more.y; ++c) join(a.cont_o, a.cont_ml, static_cast<int64_t>(more.x + c) * 256 + place);
+    const int64_t head = own * a.hkv + kvh;
+    first_ml[own] = a.main_ml[head * a.rows + at];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) first[own][i] = a.main_o[(head * 32 + quad + i) * a.rows + at];
+    const int box = own ? a.box_o : a.box_p, per = own ? a.per_o : a.per_p, from = own ? t : tok;
+    const int tile = from / box, pair = tile / per;
+    more[own] = a.info[(own ? a.hkv * (a.units_p + b * a.units_o) + kvh * a.units_o : kvh * a.units_p) + pair];
+    place[own] = (tile - pair * per) * 128 + (from - tile * box) * a.group + g;
+    len[own] = own ? sh_len(a, b) : sh_prefix(a);
+  }
+#pragma unroll
+  for (int own = 0; own < 2; ++own) {
+    if (len[own] == 0) continue;
+    join(first_ml[own], first[own]);
+    for (int c = 1; c <= more[own].y; ++c) {
+      const int64_t cta = more[own].x + c;
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a.cont_o[(cta * 32 + quad + i) * 256 + place[own]];
+      join(a.cont_ml[cta * 256 + place[own]], v);
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;             // (a NaN stays one)
-  *reinterpret_cast<uint2*>(a.out + r * kHeadDim + lane * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (a.lse != nullptr && lane == 0) a.lse[r] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  const int64_t row = static_cast<int64_t>(tok) * a.hq + kvh * a.group + g;
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = pack_bf16x2(acc[i].x * inv, acc[i].y * inv);
+    o[2 * i + 1] = pack_bf16x2(acc[i].z * inv, acc[i].w * inv);
+  }
+  uint4* dst = reinterpret_cast<uint4*>(a.out + row * kHeadDim + quad * 4);
+  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  if (a.lse != nullptr && quad == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // Tiles and units of a call.
-static void sh_units(ShArgs& a) {
+static void sh_units(ShArgs& a, int sms) {
   a.group = a.hq / a.hkv;
   a.tokens = a.bs * a.block;
+  a.rows = a.tokens * a.group;
   const int most = 128 / a.group;
   a.box_p = a.tokens < most ? a.tokens : most;
-  a.tiles_p = (a.tokens + a.box_p - 1) / a.box_p;
+  const int tiles_p = (a.tokens + a.box_p - 1) / a.box_p;
   a.box_o = a.block < most ? a.block : most;
-  a.tiles_o = (a.block + a.box_o - 1) / a.box_o;
-  a.per_p = a.tiles_p > 1 ? 2 : 1;
-  a.per_o = a.tiles_o > 1 ? 2 : 1;
-  a.units_p = (a.tiles_p + a.per_p - 1) / a.per_p;
-  a.units_o = (a.tiles_o + a.per_o - 1) / a.per_o;
+  const int tiles_o = (a.block + a.box_o - 1) / a.box_o;
+  // two tiles to a unit share the reading of the keys and the time of the products; one by one they spread over more SMs
+  a.per_p = tiles_p > 1 && static_cast<int64_t>(a.hkv) * tiles_p * a.prefix_pages * (kPage / kAtKeys) >= 4ll * sms ? 2 : 1;
+  a.per_o = tiles_o > 1 ? 2 : 1;
+  a.units_p = (tiles_p + a.per_p - 1) / a.per_p;
+  a.units_o = (tiles_o + a.per_o - 1) / a.per_o;
 }
 
 }  // namespace mdb
@@ -584,7 +683,7 @@ int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cach
   if (bs == 0) return MDB_OK;
   MDB_REQUIRE(q && k_cache && v_cache && out && block_table && ctx_lens && (prefix_pages == 0 || (prefix_table && prefix_len)), MDB_ERR_ARG);
   MDB_REQUIRE(hq / hkv <= 128 && softmax_scale > 0.f && bs <= 65535 && block <= 65535 && hq <= 65535 && num_pages <= (1 << 23) &&
-                  table_pages <= (1 << 22) && prefix_pages <= (1 << 22) && static_cast<int64_t>(bs) * block * hq <= (1ll << 30),
+                  table_pages <= (1 << 22) && prefix_pages <= (1 << 22) && static_cast<int64_t>(bs) * block * hq <= (1ll << 26),
               MDB_ERR_UNSUPPORTED);
   MDB_REQUIRE(mdb_aligned16(q) && mdb_aligned16(k_cache) && mdb_aligned16(v_cache) && mdb_aligned16(out) && mdb_aligned16(workspace), MDB_ERR_ALIGN);
   MDB_REQUIRE(workspace != nullptr && workspace_bytes >= mdb_attn_shared_workspace_bytes(bs, block, hq, hkv), MDB_ERR_WORKSPACE);
@@ -598,14 +697,17 @@ int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cach
   a.prefix_pages = prefix_pages; a.table_stride = table_stride; a.table_pages = table_pages; a.num_pages = num_pages;
   a.bs = bs; a.block = block; a.hq = hq; a.hkv = hkv;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  sh_units(a);
   const int sms = at_sm_count();
+  sh_units(a, sms);
+  // the list's length is kept in 32 bits (2^32 is minutes of work)
+  const int64_t steps = kPage / kAtKeys, most = (prefix_pages * steps * kShTwoStep + kShUnit) * a.units_p + (table_pages * steps * kShTwoStep + kShUnit) * a.units_o * bs;
+  MDB_REQUIRE(most <= 0xf0000000ll / hkv, MDB_ERR_UNSUPPORTED);
   const int64_t rows = static_cast<int64_t>(a.tokens) * hq;
-  a.main_o = static_cast<float*>(workspace);
-  a.cont_o = a.main_o + 2 * rows * kHeadDim;
-  a.main_ml = a.cont_o + static_cast<int64_t>(sms) * 256 * kHeadDim;
-  a.cont_ml = a.main_ml + 2 * rows * 2;
-  a.info = reinterpret_cast<int2*>(a.cont_ml + static_cast<int64_t>(sms) * 256 * 2);
+  a.main_o = static_cast<float4*>(workspace);
+  a.cont_o = a.main_o + 2 * rows * 32;
+  a.main_ml = reinterpret_cast<float2*>(a.cont_o + static_cast<int64_t>(sms) * 256 * 32);
+  a.cont_ml = a.main_ml + 2 * rows;
+  a.info = reinterpret_cast<int2*>(a.cont_ml + static_cast<int64_t>(sms) * 256);
   CUtensorMap map_qp, map_qo, map_k, map_v;
   if (!encode_queries(q, a.tokens, hq, a.group, a.box_p, &map_qp) || !encode_queries(q, a.tokens, hq, a.group, a.box_o, &map_qo) ||
       !encode_cache(k_cache, num_pages, hkv, &map_k) || !encode_cache(v_cache, num_pages, hkv, &map_v))
@@ -620,7 +722,7 @@ int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cach
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = mdb_launch(attn_shared_kernel, dim3(sms), dim3(ShPlan::kThreads), ShPlan::kSmemBytes, st, map_qp, map_qo, map_k, map_v, a);
   if (rc != MDB_OK) return rc;
-  return mdb_launch(attn_shared_merge, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, a);
+  return mdb_launch(attn_shared_merge, dim3((a.rows + 31) / 32, hkv), dim3(256), 0, st, a);
 }
 
 }  // extern "C"
