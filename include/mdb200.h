@@ -738,18 +738,40 @@ int mdb_rotary_embed(const mdb_rotary_embed_args* args, mdb_stream_t stream);
  * -inf.  prefix_pages 0: no prefix (prefix_table and prefix_len may be NULL).  The workspace is always needed; calls in flight at
  * the same time need one each. */
 int64_t mdb_attn_shared_workspace_bytes(int bs, int block, int hq, int hkv);
-int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int32_t* prefix_table,
-                          int prefix_pages, const int32_t* prefix_len, const int32_t* block_table, int table_stride,
-                          int table_pages, const int32_t* ctx_lens, int bs, int block, int hq, int hkv, int num_pages,
-                          float softmax_scale, void* workspace, int64_t workspace_bytes, mdb_stream_t stream);
+typedef struct {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  float* lse;
+  const int32_t* prefix_table;
+  const int32_t* prefix_len;
+  const int32_t* block_table;
+  const int32_t* ctx_lens;
+  int32_t prefix_pages, table_stride, table_pages, num_pages, bs, block, hq, hkv;
+  float softmax_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} mdb_attn_shared_args;
+int mdb_attn_block_shared(const mdb_attn_shared_args* args, mdb_stream_t stream);
 
 /* The weight every key of a request's own pages receives from a block of queries, by key head: out[b][h][j] = decay *
  * previous[b][h][j] + the sum over the block's tokens t and the heads g of group h of exp(q . k_j * softmax_scale -
  * lse[b][t][g]) for j < ctx_lens[b], 0 behind.  lse as mdb_attn_block_shared returns it (rows of -inf weigh nothing).  out and
  * previous (may be NULL: 0; may be out) fp32 [bs][hkv][cols]. */
-int mdb_key_weights(const void* q, const void* k_cache, const float* lse, const int32_t* block_table, int table_stride,
-                    int table_pages, const int32_t* ctx_lens, int bs, int block, int hq, int hkv, int num_pages, float softmax_scale,
-                    const float* previous, float decay, float* out, int64_t cols, mdb_stream_t stream);
+typedef struct {
+  const void* q;
+  const void* k_cache;
+  const float* lse;
+  const float* previous;
+  float* out;
+  const int32_t* block_table;
+  const int32_t* ctx_lens;
+  int64_t cols;
+  int32_t table_stride, table_pages, num_pages, bs, block, hq, hkv;
+  float softmax_scale, decay;
+} mdb_key_weights_args;
+int mdb_key_weights(const mdb_key_weights_args* args, mdb_stream_t stream);
 
 /* Eviction: of the seqlens[b] keys of a request the last `recent` and, by key head, the budget - recent of largest weight among those
  * in front stay (NaN counts as the lowest weight; the lowest index wins a tie); all of them where there are no more than budget.

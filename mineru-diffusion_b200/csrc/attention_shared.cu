@@ -676,41 +676,43 @@ int64_t mdb_attn_shared_workspace_bytes(int bs, int block, int hq, int hkv) {
   return (2 * rows + 256ll * at_sm_count()) * (kHeadDim + 2) * 4 + (rows / hkv + bs + 2) * static_cast<int64_t>(hkv) * 16;
 }
 
-int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int32_t* prefix_table,
-                          int prefix_pages, const int32_t* prefix_len, const int32_t* block_table, int table_stride, int table_pages, const int32_t* ctx_lens, int bs,
-                          int block, int hq, int hkv, int num_pages, float softmax_scale, void* workspace, int64_t workspace_bytes, mdb_stream_t stream) {
-  MDB_REQUIRE(bs >= 0 && block > 0 && hq > 0 && hkv > 0 && num_pages > 0 && table_pages > 0 && (table_stride >= table_pages || bs <= 1) && prefix_pages >= 0 && hq % hkv == 0, MDB_ERR_ARG);
-  if (bs == 0) return MDB_OK;
-  MDB_REQUIRE(q && k_cache && v_cache && out && block_table && ctx_lens && (prefix_pages == 0 || (prefix_table && prefix_len)), MDB_ERR_ARG);
-  MDB_REQUIRE(hq / hkv <= 128 && softmax_scale > 0.f && bs <= 65535 && block <= 65535 && hq <= 65535 && num_pages <= (1 << 23) &&
-                  table_pages <= (1 << 22) && prefix_pages <= (1 << 22) && static_cast<int64_t>(bs) * block * hq <= (1ll << 26),
+int mdb_attn_block_shared(const mdb_attn_shared_args* args, mdb_stream_t stream) {
+  MDB_REQUIRE(args != nullptr, MDB_ERR_ARG);
+  const mdb_attn_shared_args c = *args;
+  MDB_REQUIRE(c.bs >= 0 && c.block > 0 && c.hq > 0 && c.hkv > 0 && c.num_pages > 0 && c.table_pages > 0 && c.prefix_pages >= 0 && c.hq % c.hkv == 0 &&
+                  (c.table_stride >= c.table_pages || c.bs <= 1),
+              MDB_ERR_ARG);
+  if (c.bs == 0) return MDB_OK;
+  MDB_REQUIRE(c.q && c.k_cache && c.v_cache && c.out && c.block_table && c.ctx_lens && (c.prefix_pages == 0 || (c.prefix_table && c.prefix_len)), MDB_ERR_ARG);
+  MDB_REQUIRE(c.hq / c.hkv <= 128 && c.softmax_scale > 0.f && c.bs <= 65535 && c.block <= 65535 && c.hq <= 65535 && c.num_pages <= (1 << 23) &&
+                  c.table_pages <= (1 << 22) && c.prefix_pages <= (1 << 22) && static_cast<int64_t>(c.bs) * c.block * c.hq <= (1ll << 26),
               MDB_ERR_UNSUPPORTED);
-  MDB_REQUIRE(mdb_aligned16(q) && mdb_aligned16(k_cache) && mdb_aligned16(v_cache) && mdb_aligned16(out) && mdb_aligned16(workspace), MDB_ERR_ALIGN);
-  MDB_REQUIRE(workspace != nullptr && workspace_bytes >= mdb_attn_shared_workspace_bytes(bs, block, hq, hkv), MDB_ERR_WORKSPACE);
+  MDB_REQUIRE(mdb_aligned16(c.q) && mdb_aligned16(c.k_cache) && mdb_aligned16(c.v_cache) && mdb_aligned16(c.out) && mdb_aligned16(c.workspace), MDB_ERR_ALIGN);
+  MDB_REQUIRE(c.workspace != nullptr && c.workspace_bytes >= mdb_attn_shared_workspace_bytes(c.bs, c.block, c.hq, c.hkv), MDB_ERR_WORKSPACE);
   ShArgs a = {};
-  a.out = static_cast<bf16*>(out);
-  a.lse = lse;
-  a.prefix_len = prefix_pages > 0 ? prefix_len : nullptr;
-  a.prefix_table = prefix_table;
-  a.ctx_lens = ctx_lens;
-  a.block_table = block_table;
-  a.prefix_pages = prefix_pages; a.table_stride = table_stride; a.table_pages = table_pages; a.num_pages = num_pages;
-  a.bs = bs; a.block = block; a.hq = hq; a.hkv = hkv;
-  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.out = static_cast<bf16*>(c.out);
+  a.lse = c.lse;
+  a.prefix_len = c.prefix_pages > 0 ? c.prefix_len : nullptr;
+  a.prefix_table = c.prefix_table;
+  a.ctx_lens = c.ctx_lens;
+  a.block_table = c.block_table;
+  a.prefix_pages = c.prefix_pages; a.table_stride = c.table_stride; a.table_pages = c.table_pages; a.num_pages = c.num_pages;
+  a.bs = c.bs; a.block = c.block; a.hq = c.hq; a.hkv = c.hkv;
+  a.scale_log2 = c.softmax_scale * 1.4426950408889634f;
   const int sms = at_sm_count();
   sh_units(a, sms);
   // the list's length is kept in 32 bits (2^32 is minutes of work)
-  const int64_t steps = kPage / kAtKeys, most = (prefix_pages * steps * kShTwoStep + kShUnit) * a.units_p + (table_pages * steps * kShTwoStep + kShUnit) * a.units_o * bs;
-  MDB_REQUIRE(most <= 0xf0000000ll / hkv, MDB_ERR_UNSUPPORTED);
-  const int64_t rows = static_cast<int64_t>(a.tokens) * hq;
-  a.main_o = static_cast<float4*>(workspace);
+  const int64_t steps = kPage / kAtKeys, most = (a.prefix_pages * steps * kShTwoStep + kShUnit) * a.units_p + (a.table_pages * steps * kShTwoStep + kShUnit) * a.units_o * a.bs;
+  MDB_REQUIRE(most <= 0xf0000000ll / a.hkv, MDB_ERR_UNSUPPORTED);
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.hq;
+  a.main_o = static_cast<float4*>(c.workspace);
   a.cont_o = a.main_o + 2 * rows * 32;
   a.main_ml = reinterpret_cast<float2*>(a.cont_o + static_cast<int64_t>(sms) * 256 * 32);
   a.cont_ml = a.main_ml + 2 * rows;
   a.info = reinterpret_cast<int2*>(a.cont_ml + static_cast<int64_t>(sms) * 256);
   CUtensorMap map_qp, map_qo, map_k, map_v;
-  if (!encode_queries(q, a.tokens, hq, a.group, a.box_p, &map_qp) || !encode_queries(q, a.tokens, hq, a.group, a.box_o, &map_qo) ||
-      !encode_cache(k_cache, num_pages, hkv, &map_k) || !encode_cache(v_cache, num_pages, hkv, &map_v))
+  if (!encode_queries(c.q, a.tokens, a.hq, a.group, a.box_p, &map_qp) || !encode_queries(c.q, a.tokens, a.hq, a.group, a.box_o, &map_qo) ||
+      !encode_cache(c.k_cache, a.num_pages, a.hkv, &map_k) || !encode_cache(c.v_cache, a.num_pages, a.hkv, &map_v))
     return MDB_ERR_CUDA;
   static PerDeviceOnce attr_once;
   const int dev = attr_once.slot();
@@ -722,7 +724,7 @@ int mdb_attn_block_shared(const void* q, const void* k_cache, const void* v_cach
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = mdb_launch(attn_shared_kernel, dim3(sms), dim3(ShPlan::kThreads), ShPlan::kSmemBytes, st, map_qp, map_qo, map_k, map_v, a);
   if (rc != MDB_OK) return rc;
-  return mdb_launch(attn_shared_merge, dim3((a.rows + 31) / 32, hkv), dim3(256), 0, st, a);
+  return mdb_launch(attn_shared_merge, dim3((a.rows + 31) / 32, a.hkv), dim3(256), 0, st, a);
 }
 
 }  // extern "C"

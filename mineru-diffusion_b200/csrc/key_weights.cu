@@ -318,25 +318,27 @@ static bool encode_cache(const void* cache, int num_pages, int hkv, CUtensorMap*
 
 using namespace mdb;
 
-extern "C" int mdb_key_weights(const void* q, const void* k_cache, const float* lse, const int32_t* block_table, int table_stride, int table_pages,
-                               const int32_t* ctx_lens, int bs, int block, int hq, int hkv, int num_pages, float softmax_scale,
-                               const float* previous, float decay, float* out, int64_t cols, mdb_stream_t stream) {
-  MDB_REQUIRE(bs >= 0 && block > 0 && hq > 0 && hkv > 0 && num_pages > 0 && table_pages > 0 && (table_stride >= table_pages || bs <= 1) && cols > 0 && hq % hkv == 0, MDB_ERR_ARG);
-  if (bs == 0) return MDB_OK;
-  MDB_REQUIRE(q && k_cache && lse && block_table && ctx_lens && out, MDB_ERR_ARG);
-  MDB_REQUIRE(mdb_aligned16(q) && mdb_aligned16(k_cache), MDB_ERR_ALIGN);
-  const int group = hq / hkv;
-  MDB_REQUIRE(bs <= 65535 && block <= 65535 && group <= 128 && num_pages <= (1 << 23) && table_pages <= (1 << 22) && cols <= (1ll << 30) &&
-                  static_cast<int64_t>(bs) * block <= (1ll << 30) && softmax_scale > 0.f && hq <= 65535,
+extern "C" int mdb_key_weights(const mdb_key_weights_args* args, mdb_stream_t stream) {
+  MDB_REQUIRE(args != nullptr, MDB_ERR_ARG);
+  const mdb_key_weights_args w = *args;
+  MDB_REQUIRE(w.bs >= 0 && w.block > 0 && w.hq > 0 && w.hkv > 0 && w.num_pages > 0 && w.table_pages > 0 && w.cols > 0 && w.hq % w.hkv == 0 &&
+                  (w.table_stride >= w.table_pages || w.bs <= 1),
+              MDB_ERR_ARG);
+  if (w.bs == 0) return MDB_OK;
+  MDB_REQUIRE(w.q && w.k_cache && w.lse && w.block_table && w.ctx_lens && w.out, MDB_ERR_ARG);
+  MDB_REQUIRE(mdb_aligned16(w.q) && mdb_aligned16(w.k_cache), MDB_ERR_ALIGN);
+  const int group = w.hq / w.hkv;
+  MDB_REQUIRE(w.bs <= 65535 && w.block <= 65535 && group <= 128 && w.num_pages <= (1 << 23) && w.table_pages <= (1 << 22) && w.cols <= (1ll << 30) &&
+                  static_cast<int64_t>(w.bs) * w.block <= (1ll << 30) && w.softmax_scale > 0.f && w.hq <= 65535,
               MDB_ERR_UNSUPPORTED);
   KwArgs a = {};
-  a.lse = lse; a.previous = previous; a.out = out;
-  a.block_table = block_table; a.seqlens = ctx_lens;
-  a.bs = bs; a.block = block; a.hq = hq; a.hkv = hkv; a.group = group;
-  a.table_stride = table_stride; a.table_pages = table_pages; a.num_pages = num_pages; a.cols = cols;
-  a.scale_log2 = softmax_scale * 1.4426950408889634f; a.decay = decay;
-  a.tokens = block < kKwMaxRows / group ? block : kKwMaxRows / group;
-  a.row_blocks = (block + a.tokens - 1) / a.tokens;
+  a.lse = w.lse; a.previous = w.previous; a.out = w.out;
+  a.block_table = w.block_table; a.seqlens = w.ctx_lens;
+  a.bs = w.bs; a.block = w.block; a.hq = w.hq; a.hkv = w.hkv; a.group = group;
+  a.table_stride = w.table_stride; a.table_pages = w.table_pages; a.num_pages = w.num_pages; a.cols = w.cols;
+  a.scale_log2 = w.softmax_scale * 1.4426950408889634f; a.decay = w.decay;
+  a.tokens = w.block < kKwMaxRows / group ? w.block : kKwMaxRows / group;
+  a.row_blocks = (w.block + a.tokens - 1) / a.tokens;
   a.n_pad = (a.tokens * group + 15) / 16 * 16;
   a.q_bufs = a.n_pad > 128 && a.row_blocks == 1 ? 1 : 2;        // (room for key tiles; the rows change once in a run)
   const int rest = 1024 + 8 * kKwMaxRows * 4 + (a.row_blocks > 1 ? kKwSegTiles * kAtKeys * 4 : 0) + 8 * kKwBarCount + 16;
@@ -344,7 +346,7 @@ extern "C" int mdb_key_weights(const void* q, const void* k_cache, const float* 
   if (a.stages > kKwMaxStages) a.stages = kKwMaxStages;
   const int smem = rest + a.q_bufs * a.n_pad * 256 + a.stages * kAtTileBytes;
   CUtensorMap map_q, map_k;
-  if (!encode_queries(q, static_cast<int64_t>(bs) * block, hq, group, a.tokens, &map_q) || !encode_cache(k_cache, num_pages, hkv, &map_k))
+  if (!encode_queries(w.q, static_cast<int64_t>(w.bs) * w.block, w.hq, group, a.tokens, &map_q) || !encode_cache(w.k_cache, w.num_pages, w.hkv, &map_k))
     return MDB_ERR_CUDA;
   static PerDeviceOnce attr_once;
   const int dev = attr_once.slot();
@@ -353,8 +355,8 @@ extern "C" int mdb_key_weights(const void* q, const void* k_cache, const float* 
     if (cudaFuncSetAttribute(key_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKwSmem) != cudaSuccess) return MDB_ERR_CUDA;
     attr_once.done[dev] = true;
   }
-  const int64_t most = cols < static_cast<int64_t>(table_pages) * kPage ? cols : static_cast<int64_t>(table_pages) * kPage;
-  const int64_t tiles = (most + kAtKeys - 1) / kAtKeys * bs * hkv;
+  const int64_t table = static_cast<int64_t>(w.table_pages) * kPage, most = w.cols < table ? w.cols : table;
+  const int64_t tiles = (most + kAtKeys - 1) / kAtKeys * w.bs * w.hkv;
   const int sms = at_sm_count();
   return mdb_launch(key_weights_kernel, dim3(tiles < sms ? static_cast<int>(tiles) : sms), dim3(kKwThreads), smem, static_cast<cudaStream_t>(stream),
                     map_q, map_k, a);

@@ -910,18 +910,17 @@ def copy_rows(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor) -> torc
 # Long contexts: rotary positions of any layout and scaling, attention behind a shared prefix, the weights of its keys and the
 # eviction that goes by them.
 
-def _here(**tensors) -> None:
+_current_device = _device or torch.cuda.current_device
+_pack_rotary, _pack_shared, _pack_weights, _pack_evict = (_lib.packer(b) for b in (
+    _lib.RotaryEmbedArgs, _lib.AttnSharedArgs, _lib.KeyWeightsArgs, _lib.KvEvictArgs))
+
+
+def _all_here(*tensors) -> None:
     """All tensors (None: absent) on the current CUDA device: kernels are launched there."""
-    dev = torch.cuda.current_device() if _device is None else None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{name} must be a CUDA tensor (libmdb200 has no CPU path)")
-        if dev is None:
-            dev = _device()
-        if t.get_device() != dev:
-            raise RuntimeError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{dev}")
+    here = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise RuntimeError(f"a tensor is on {t.device}, the current device is cuda:{here} (libmdb200 has no CPU path)")
 
 
 def rope_frequencies(rot_dims: int, base: float = 10000.0, scaling: dict | None = None, device="cuda") -> tuple[torch.Tensor, float]:
@@ -963,10 +962,12 @@ def rope_frequencies(rot_dims: int, base: float = 10000.0, scaling: dict | None 
     return torch.tensor(f, dtype=torch.float64, device=device), factor
 
 
-def _heads_of(t: torch.Tensor, n: int, d: int, dtype, name: str) -> int:
-    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != d or t.stride(2) != 1 or t.dtype != dtype:
-        raise ValueError(f"{name} must be [{n}, heads, {d}] of {dtype} with a dense last dimension")
-    return t.shape[1]
+def _heads_strides(t: torch.Tensor, n: int, d: int, dtype, name: str, heads: int | None = None) -> tuple:
+    """(heads, row stride, head stride) of t [n, heads, d]."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != n or shape[2] != d or strides[2] != 1 or t.dtype is not dtype or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [{n}, {heads or 'heads'}, {d}] of {dtype} with a dense last dimension")
+    return shape[1], strides[0], strides[1]
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
@@ -979,50 +980,79 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     ``inverse`` turns back, which is also the gradient with respect to the input.  ``q_out`` / ``k_out`` may be the inputs.
     With ``slot_mapping`` (int32 [n], -1 = skip) the keys, and ``v`` if given, go to those rows of the caches [pages, 256, hkv, d]
     as ``store_kvcache`` puts them there.  Returns (q_out, k_out or None)."""
-    if q.dim() != 3:
-        raise ValueError("q must be [n, heads, dim]")
-    n, hq, d = q.shape
-    _here(q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, q_out=q_out, k_out=k_out, k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
-    dtype = _act_dtype(q, "q")
-    _heads_of(q, n, d, q.dtype, "q")
-    if positions.dtype != torch.int64 or positions.numel() != n or not positions.is_contiguous():
+    n, _, d = q.shape
+    dtype = q.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"q must be bfloat16 or float32, got {dtype}")
+    _all_here(q, k, positions, inv_freq, q_out, k_out, v, k_cache, v_cache, slot_mapping)
+    hq, q_row, q_head = _heads_strides(q, n, d, dtype, "q")
+    if positions.dtype is not torch.int64 or positions.numel() != n or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int64 tensor with one entry per row")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > d:
+    pairs = inv_freq.numel()
+    if inv_freq.dtype is not torch.float64 or 2 * pairs > d or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 vector of at most half as many entries as a head has channels")
     if q_out is None:
-        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-    elif _heads_of(q_out, n, d, q.dtype, "q_out") != hq:
-        raise ValueError("q_out must have the shape of q")
-    hkv = 0 if k is None else _heads_of(k, n, d, q.dtype, "k")
-    a = _lib.RotaryEmbedArgs(dtype, n, hq, hkv, d, 2 * inv_freq.numel(), int(interleaved), int(inverse))
-    a.q, a.q_row, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
-    a.q_out, a.q_out_row, a.q_out_head = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
-    a.positions, a.inv_freq, a.scale = positions.data_ptr(), inv_freq.data_ptr(), scale
+        q_out = q.new_empty((n, hq, d))
+        qo_row, qo_head = hq * d, d
+    else:
+        _, qo_row, qo_head = _heads_strides(q_out, n, d, dtype, "q_out", hq)
+    hkv, k_row, k_head = (0, 0, 0) if k is None else _heads_strides(k, n, d, dtype, "k")
+    v_row = v_head = ko_row = ko_head = slots = 0
     if slot_mapping is not None:
         if k is None or k_cache is None or (v is None) != (v_cache is None) or k_out is not None:
             raise ValueError("a store needs k and k_cache, v and v_cache together, and no k_out")
-        if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != n or not slot_mapping.is_contiguous():
+        if slot_mapping.dtype is not torch.int32 or slot_mapping.numel() != n or not slot_mapping.is_contiguous():
             raise ValueError("slot_mapping must be a contiguous int32 tensor with one entry per row")
-        for c, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            if c is not None and (c.dim() != 4 or c.shape[2] != hkv or c.shape[3] != d or c.dtype != q.dtype or not c.is_contiguous()):
-                raise ValueError(f"{nm} must be contiguous [pages, 256, {hkv}, {d}] of {q.dtype}")
+        shape = k_cache.shape
+        if len(shape) != 4 or shape[2] != hkv or shape[3] != d or k_cache.dtype is not dtype or not k_cache.is_contiguous():
+            raise ValueError(f"k_cache must be contiguous [pages, 256, {hkv}, {d}] of {dtype}")
         if v is not None:
-            if _heads_of(v, n, d, q.dtype, "v") != hkv or v_cache.shape != k_cache.shape:
-                raise ValueError("v must have the shape of k, and the caches the same shape")
-            a.v, a.v_row, a.v_head, a.v_cache = v.data_ptr(), v.stride(0), v.stride(1), v_cache.data_ptr()
-        a.slots, a.num_slots, a.k_cache = slot_mapping.data_ptr(), k_cache.shape[0] * k_cache.shape[1], k_cache.data_ptr()
+            _, v_row, v_head = _heads_strides(v, n, d, dtype, "v", hkv)
+            if v_cache.shape != shape or v_cache.dtype is not dtype or not v_cache.is_contiguous():
+                raise ValueError("v_cache must be contiguous, of the type and shape of k_cache")
+        slots = shape[0] * shape[1]
     elif v is not None or k_cache is not None or v_cache is not None:
         raise ValueError("v and the caches go with a slot_mapping")
-    elif k is not None:
-        if k_out is None:
-            k_out = torch.empty((n, hkv, d), dtype=q.dtype, device=q.device)
-        elif _heads_of(k_out, n, d, q.dtype, "k_out") != hkv:
-            raise ValueError("k_out must have the shape of k")
-        a.k_out, a.k_out_row, a.k_out_head = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
-    if k is not None:
-        a.k, a.k_row, a.k_head = k.data_ptr(), k.stride(0), k.stride(1)
-    _lib.check(_lib.lib().mdb_rotary_embed(a, _stream()), "mdb_rotary_embed")
+    elif k is None:
+        if k_out is not None:
+            raise ValueError("k_out goes with k")
+    elif k_out is None:
+        k_out = q.new_empty((n, hkv, d))
+        ko_row, ko_head = hkv * d, d
+    else:
+        _, ko_row, ko_head = _heads_strides(k_out, n, d, dtype, "k_out", hkv)
+    block = _pack_rotary(
+        code, n, hq, hkv, d, 2 * pairs, bool(interleaved), bool(inverse), q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(),
+        q_row, q_head, k_row, k_head, v_row, v_head, positions.data_ptr(), inv_freq.data_ptr(), 0 if slot_mapping is None else slot_mapping.data_ptr(), slots,
+        q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), qo_row, qo_head, ko_row, ko_head, 0 if k_cache is None else k_cache.data_ptr(),
+        0 if v_cache is None else v_cache.data_ptr(), scale)
+    _lib.check(_lib.lib().mdb_rotary_embed(block, _stream()), "mdb_rotary_embed")
     return q_out, k_out
+
+
+def _table_args(table: torch.Tensor, bs: int) -> tuple:
+    """(row stride, pages per row) of a page table."""
+    shape, strides = table.shape, table.stride()
+    if len(shape) != 2 or shape[0] < bs or table.dtype is not torch.int32 or (shape[1] > 1 and strides[1] != 1):
+        raise ValueError("page tables must be int32 [bs, pages per request] with unit stride inside a row")
+    return strides[0], shape[1]
+
+
+def _paged_args(q, k_cache, cache_seqlens, block_table) -> tuple:
+    """The checks of ``_block_attn_args`` for one cache."""
+    bs, block, hq, d = q.shape
+    pages, page, hkv, d2 = k_cache.shape
+    if d != 128 or d2 != 128 or page != 256:
+        raise ValueError("head_dim must be 128 and pages 256 tokens")
+    if q.dtype is not _BF16 or k_cache.dtype is not _BF16:
+        raise TypeError("q and the caches must be bfloat16")
+    if not (q.is_contiguous() and k_cache.is_contiguous()):
+        raise ValueError("q and the caches must be contiguous")
+    if cache_seqlens.dtype is not torch.int32 or cache_seqlens.numel() < bs or not cache_seqlens.is_contiguous():
+        raise ValueError("cache_seqlens must hold one contiguous int32 per request")
+    stride, table_pages = _table_args(block_table, bs)
+    return bs, block, hq, hkv, pages, d, stride, table_pages
 
 
 def shared_prefix_workspace_bytes(bs: int, block: int, hq: int, hkv: int) -> int:
@@ -1040,33 +1070,40 @@ def block_attn_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     gets zeros.  Returns out, or (out, lse) with ``want_lse`` or ``lse`` (fp32 [bs, B, Hq], the logarithm of the softmax's
     denominator, -inf where there is no key): what ``key_weights`` takes.  Calls in flight at the same time need a ``workspace``
     (``shared_prefix_workspace_bytes``) each."""
-    _here(q=q, k_cache=k_cache, v_cache=v_cache, prefix_seqlen=prefix_seqlen, prefix_table=prefix_table, cache_seqlens=cache_seqlens,
-          block_table=block_table, workspace=workspace, out=out, lse=lse)
-    bs, block, hq, hkv, pages, d = _block_attn_args(q, k_cache, v_cache, cache_seqlens, block_table, out)
-    prefix_pages = 0
+    _all_here(q, k_cache, v_cache, prefix_seqlen, prefix_table, cache_seqlens, block_table, workspace, out, lse)
+    bs, block, hq, hkv, pages, d, stride, table_pages = _paged_args(q, k_cache, cache_seqlens, block_table)
+    if v_cache.shape != k_cache.shape or v_cache.dtype is not _BF16 or not v_cache.is_contiguous():
+        raise ValueError("v_cache must be contiguous, of the type and shape of k_cache")
     if (prefix_table is None) != (prefix_seqlen is None):
         raise ValueError("prefix_seqlen and prefix_table go together")
+    prefix_pages = 0
     if prefix_table is not None:
         prefix_pages = prefix_table.numel()
-        if prefix_table.dtype != torch.int32 or not prefix_table.is_contiguous():
+        if prefix_table.dtype is not torch.int32 or not prefix_table.is_contiguous():
             raise ValueError("prefix_table must be a contiguous int32 list of pages")
-        if prefix_seqlen.dtype != torch.int32 or prefix_seqlen.numel() != 1:
+        if prefix_seqlen.dtype is not torch.int32 or prefix_seqlen.numel() != 1:
             raise ValueError("prefix_seqlen must be one int32")
-    if softmax_scale is None:
-        softmax_scale = d ** -0.5
     if out is None:
         out = torch.empty_like(q)
-    if lse is None:
-        lse = torch.empty((bs, block, hq), dtype=torch.float32, device=q.device) if want_lse else None
-    elif lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
-        raise ValueError("lse must be a contiguous fp32 [bs, block, Hq]")
-    need = _lib.lib().mdb_attn_shared_workspace_bytes(bs, block, hq, hkv)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _lib.check(_lib.lib().mdb_attn_block_shared(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(prefix_table), prefix_pages, _ptr(prefix_seqlen),
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cache_seqlens.data_ptr(), bs, block, hq, hkv, pages, float(softmax_scale),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()), "mdb_attn_block_shared")
+    elif out.shape != q.shape or out.dtype is not _BF16 or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of the type and shape of q")
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
+            raise ValueError("lse must be a contiguous fp32 [bs, block, Hq]")
+    elif want_lse:
+        lse = q.new_empty((bs, block, hq), dtype=torch.float32)
+    lib = _lib.lib()
+    if workspace is None:
+        room = lib.mdb_attn_shared_workspace_bytes(bs, block, hq, hkv)
+        workspace = q.new_empty(room, dtype=torch.uint8)
+    else:
+        room = workspace.numel() * workspace.element_size()
+    args = _pack_shared(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        0 if prefix_table is None else prefix_table.data_ptr(), 0 if prefix_seqlen is None else prefix_seqlen.data_ptr(), block_table.data_ptr(),
+        cache_seqlens.data_ptr(), prefix_pages, stride, table_pages, pages, bs, block, hq, hkv, d ** -0.5 if softmax_scale is None else softmax_scale,
+        workspace.data_ptr(), room)
+    _lib.check(lib.mdb_attn_block_shared(args, _stream()), "mdb_attn_block_shared")
     return out if lse is None else (out, lse)
 
 
@@ -1078,20 +1115,20 @@ def key_weights(q: torch.Tensor, k_cache: torch.Tensor, lse: torch.Tensor, cache
     j < cache_seqlens[b]; 0 behind.  ``lse`` is what the attention over all keys returned (``block_attn_shared_prefix``); q and the
     caches as there.  For a prefix's keys, pass the batch as one request: q.view(1, bs * B, Hq, 128), its table and length.
     ``previous`` may be ``out``; without either there are as many columns as the page table addresses."""
-    _here(q=q, k_cache=k_cache, lse=lse, cache_seqlens=cache_seqlens, block_table=block_table, previous=previous, out=out)
-    bs, block, hq, hkv, pages, d = _block_attn_args(q, k_cache, k_cache, cache_seqlens, block_table, None)
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
+    _all_here(q, k_cache, lse, cache_seqlens, block_table, previous, out)
+    bs, block, hq, hkv, pages, d, stride, table_pages = _paged_args(q, k_cache, cache_seqlens, block_table)
+    if lse.dtype is not torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous fp32 [bs, block, Hq]")
-    cols = block_table.shape[1] * 256 if out is None and previous is None else (previous if out is None else out).shape[-1]
-    for t, nm in ((previous, "previous"), (out, "out")):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (bs, hkv, cols) or not t.is_contiguous()):
-            raise ValueError(f"{nm} must be contiguous fp32 [{bs}, {hkv}, {cols}]")
+    cols = out.shape[-1] if out is not None else previous.shape[-1] if previous is not None else table_pages * 256
+    for t in (previous, out):
+        if t is not None and (t.shape != (bs, hkv, cols) or t.dtype is not torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"previous and out must be contiguous fp32 [{bs}, {hkv}, {cols}]")
     if out is None:
-        out = torch.empty((bs, hkv, cols), dtype=torch.float32, device=q.device)
-    _lib.check(_lib.lib().mdb_key_weights(
-        q.data_ptr(), k_cache.data_ptr(), lse.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        cache_seqlens.data_ptr(), bs, block, hq, hkv, pages, float(d ** -0.5 if softmax_scale is None else softmax_scale), _ptr(previous), float(decay), out.data_ptr(), cols, _stream()),
-        "mdb_key_weights")
+        out = lse.new_empty((bs, hkv, cols)) if previous is None else torch.empty_like(previous)
+    args = _pack_weights(
+        q.data_ptr(), k_cache.data_ptr(), lse.data_ptr(), 0 if previous is None else previous.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+        cache_seqlens.data_ptr(), cols, stride, table_pages, pages, bs, block, hq, hkv, d ** -0.5 if softmax_scale is None else softmax_scale, decay)
+    _lib.check(_lib.lib().mdb_key_weights(args, _stream()), "mdb_key_weights")
     return out
 
 
@@ -1105,41 +1142,42 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.T
     prefix's); written pages must belong to one request.  Returns (kept int32 [bs, Hkv, budget] = old places, -1 behind the last;
     new lengths int32 [bs]; weights of the kept keys [bs, Hkv, >= budget], 0 behind the last).  ``weights_out`` may be ``weights`` and
     ``seqlens_out`` may be ``cache_seqlens``."""
-    _here(k_cache=k_cache, v_cache=v_cache, weights=weights, cache_seqlens=cache_seqlens, block_table=block_table, out_table=out_table,
-          weights_out=weights_out, seqlens_out=seqlens_out, kept=kept)
-    _act_dtype(k_cache, "k_cache")
-    if k_cache.dim() != 4 or k_cache.shape[1] != 256 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+    _all_here(k_cache, v_cache, weights, cache_seqlens, block_table, out_table, weights_out, seqlens_out, kept)
+    if k_cache.dtype not in _DTYPES:
+        raise TypeError(f"k_cache must be bfloat16 or float32, got {k_cache.dtype}")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[1] != 256 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
         raise ValueError("the caches must be [pages, 256, Hkv, dim] of one type and shape")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
-    pages, _, hkv, d = k_cache.shape
-    if weights.dim() != 3 or weights.dtype != torch.float32 or weights.shape[1] != hkv or weights.stride(2) != 1:
+    pages, _, hkv, d = shape
+    bs, heads, cols = weights.shape
+    w_row, w_head, w_col = weights.stride()
+    if heads != hkv or weights.dtype is not torch.float32 or w_col != 1:
         raise ValueError("weights must be fp32 [bs, Hkv, columns] with a dense last dimension")
-    bs = weights.shape[0]
     if not 0 <= recent <= budget or budget < 1:
         raise ValueError("budget must be positive and recent between 0 and budget")
-    for t, nm in ((block_table, "block_table"), (out_table, "out_table")):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] < bs or (t.shape[1] > 1 and t.stride(1) != 1)):
-            raise ValueError(f"{nm} must be int32 [bs, pages per request] with unit stride inside a row")
-    if out_table is not None and out_table.shape[1] * 256 < min(budget, block_table.shape[1] * 256):
+    stride, table_pages = _table_args(block_table, bs)
+    out_stride, out_pages = (0, 0) if out_table is None else _table_args(out_table, bs)
+    if out_table is not None and out_pages * 256 < min(budget, table_pages * 256):
         raise ValueError("out_table must have pages for budget keys")
-    for t, nm in ((cache_seqlens, "cache_seqlens"), (seqlens_out, "seqlens_out")):
-        if t is not None and (t.dtype != torch.int32 or t.numel() < bs or not t.is_contiguous()):
-            raise ValueError(f"{nm} must hold one contiguous int32 per request")
+    for t in (cache_seqlens, seqlens_out):
+        if t is not None and (t.dtype is not torch.int32 or t.numel() < bs or not t.is_contiguous()):
+            raise ValueError("cache_seqlens and seqlens_out must hold one contiguous int32 per request")
     if weights_out is None:
-        weights_out = torch.empty((bs, hkv, budget), dtype=torch.float32, device=weights.device)
-    elif weights_out.dim() != 3 or weights_out.dtype != torch.float32 or weights_out.shape[:2] != (bs, hkv) or weights_out.shape[2] < budget or weights_out.stride(2) != 1:
+        weights_out = weights.new_empty((bs, hkv, budget))
+    elif weights_out.dim() != 3 or weights_out.dtype is not torch.float32 or weights_out.shape[:2] != (bs, hkv) or weights_out.shape[2] < budget or weights_out.stride(2) != 1:
         raise ValueError("weights_out must be fp32 [bs, Hkv, at least budget] with a dense last dimension")
     if seqlens_out is None:
-        seqlens_out = torch.empty(bs, dtype=torch.int32, device=weights.device)
+        seqlens_out = cache_seqlens.new_empty(bs)
     if kept is None:
-        kept = torch.empty((bs, hkv, budget), dtype=torch.int32, device=weights.device)
-    elif kept.shape != (bs, hkv, budget) or kept.dtype != torch.int32 or not kept.is_contiguous():
+        kept = cache_seqlens.new_empty((bs, hkv, budget))
+    elif kept.shape != (bs, hkv, budget) or kept.dtype is not torch.int32 or not kept.is_contiguous():
         raise ValueError("kept must be contiguous int32 [bs, Hkv, budget]")
-    a = _lib.KvEvictArgs(bs, hkv, d * k_cache.element_size(), budget, recent, pages, block_table.stride(0), block_table.shape[1],
-                         0 if out_table is None else out_table.stride(0), 0 if out_table is None else out_table.shape[1],
-                         k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2],
-                         weights_out.data_ptr(), weights_out.stride(0), weights_out.stride(1), cache_seqlens.data_ptr(), seqlens_out.data_ptr(),
-                         block_table.data_ptr(), _ptr(out_table), kept.data_ptr())
-    _lib.check(_lib.lib().mdb_kv_evict(a, _stream()), "mdb_kv_evict")
+    o_row, o_head, _ = weights_out.stride()
+    args = _pack_evict(
+        bs, hkv, d * k_cache.element_size(), budget, recent, pages, stride, table_pages, out_stride, out_pages, k_cache.data_ptr(), v_cache.data_ptr(),
+        weights.data_ptr(), w_row, w_head, cols, weights_out.data_ptr(), o_row, o_head, cache_seqlens.data_ptr(), seqlens_out.data_ptr(),
+        block_table.data_ptr(), 0 if out_table is None else out_table.data_ptr(), kept.data_ptr())
+    _lib.check(_lib.lib().mdb_kv_evict(args, _stream()), "mdb_kv_evict")
     return kept, seqlens_out, weights_out

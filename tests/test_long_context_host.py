@@ -53,23 +53,33 @@ def test_frequencies_refused(built):
 
 def test_c_entries_refuse_before_any_launch(built):
     lib, at = built._lib.lib(), 64
-    shared = lambda **o: lib.mdb_attn_block_shared(*[{**dict(   # noqa: E731
-        q=at, k=at, v=at, out=at, lse=None, prefix=at, prefix_pages=2, prefix_len=at, table=at, stride=4, pages=4, lens=at, bs=2, block=8, hq=4, hkv=2,
-        num_pages=10, scale=0.1, ws=at, bytes=1 << 40, stream=None), **o}[n] for n in (
-            "q", "k", "v", "out", "lse", "prefix", "prefix_pages", "prefix_len", "table", "stride", "pages", "lens", "bs", "block", "hq", "hkv", "num_pages",
-            "scale", "ws", "bytes", "stream")])
-    assert shared(bs=0) == 0
-    for o, code in (({"q": None}, -1), ({"prefix": None}, -1), ({"prefix_len": None}, -1), ({"hq": 5}, -1), ({"stride": 3}, -1), ({"pages": 0}, -1), ({"bs": -1}, -1),
-                    ({"k": 72}, -2), ({"ws": 72}, -2), ({"hq": 258}, -3), ({"scale": 0.0}, -3), ({"bs": 70000}, -3), ({"scale": float("nan")}, -3),
-                    ({"bytes": 100}, -5), ({"ws": None}, -5)):
+
+    def shared(**o):
+        a = built._lib.AttnSharedArgs(prefix_pages=2, table_stride=4, table_pages=4, num_pages=10, bs=2, block=8, hq=4, hkv=2, softmax_scale=0.1,
+                                      workspace_bytes=1 << 40)
+        for n in ("q", "k_cache", "v_cache", "out", "prefix_table", "prefix_len", "block_table", "ctx_lens", "workspace"):
+            setattr(a, n, at)
+        for n, v in o.items():
+            setattr(a, n, v)
+        return lib.mdb_attn_block_shared(ctypes.byref(a), None)
+
+    assert shared(bs=0) == 0 and lib.mdb_attn_block_shared(None, None) == -1
+    for o, code in (({"q": None}, -1), ({"prefix_table": None}, -1), ({"prefix_len": None}, -1), ({"hq": 5}, -1), ({"table_stride": 3}, -1), ({"table_pages": 0}, -1),
+                    ({"bs": -1}, -1), ({"k_cache": 72}, -2), ({"workspace": 72}, -2), ({"hq": 258}, -3), ({"softmax_scale": 0.0}, -3), ({"bs": 70000}, -3),
+                    ({"softmax_scale": float("nan")}, -3), ({"workspace_bytes": 100}, -5), ({"workspace": None}, -5)):
         assert shared(**o) == code, o
-    weights = lambda **o: lib.mdb_key_weights(*[{**dict(   # noqa: E731
-        q=at, k=at, lse=at, table=at, stride=4, pages=4, lens=at, bs=2, block=8, hq=4, hkv=2, num_pages=10, scale=0.1, previous=None, decay=1.0, out=at,
-        cols=100, stream=None), **o}[n] for n in ("q", "k", "lse", "table", "stride", "pages", "lens", "bs", "block", "hq", "hkv", "num_pages", "scale",
-                                                  "previous", "decay", "out", "cols", "stream")])
-    assert weights(bs=0) == 0
-    for o, code in (({"lse": None}, -1), ({"out": None}, -1), ({"cols": 0}, -1), ({"hq": 3}, -1), ({"stride": 1}, -1), ({"q": 72}, -2), ({"hq": 258}, -3), ({"scale": -1.0}, -3),
-                    ({"cols": 1 << 40}, -3)):
+
+    def weights(**o):
+        a = built._lib.KeyWeightsArgs(cols=100, table_stride=4, table_pages=4, num_pages=10, bs=2, block=8, hq=4, hkv=2, softmax_scale=0.1, decay=1.0)
+        for n in ("q", "k_cache", "lse", "out", "block_table", "ctx_lens"):
+            setattr(a, n, at)
+        for n, v in o.items():
+            setattr(a, n, v)
+        return lib.mdb_key_weights(ctypes.byref(a), None)
+
+    assert weights(bs=0) == 0 and lib.mdb_key_weights(None, None) == -1
+    for o, code in (({"lse": None}, -1), ({"out": None}, -1), ({"cols": 0}, -1), ({"hq": 3}, -1), ({"table_stride": 1}, -1), ({"q": 72}, -2), ({"hq": 258}, -3),
+                    ({"softmax_scale": -1.0}, -3), ({"cols": 1 << 40}, -3)):
         assert weights(**o) == code, o
 
     def evict(**o):
