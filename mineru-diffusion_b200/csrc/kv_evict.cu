@@ -6,29 +6,34 @@
 //
 //   evict_select_kernel   a CTA per (request, key head).  Radix selection over the weights' bits in order (11, 11 and 10 bits, counts in
 //                         shared memory): after it the key of the last one that stays is known, and how many of its equals do.
-//                         Then one walk in order: 8 neighbouring weights per thread, sums over the CTA, places written.
-//   evict_move_kernel     rows of K and V.  To other pages: any order, chunks of rows per CTA.  In place a row's new place is never
-//                         behind its old one, so a CTA that has a slice of the channels of all rows walks them in order, loads
-//                         of a step in front of its stores.
+//                         Then the places in order, from sums over the CTA.  Up to 32768 weights stay in registers, 32 a thread.
+//   evict_move_kernel     rows of K and V, a row's places looked up once for all its pieces.  To other pages: any order, 256 rows per
+//                         CTA, all heads of a stretch of tokens side by side (they lie side by side in memory).  In place a row's
+//                         new place is never behind its old one, so a CTA that has a slice of the channels of all rows walks
+//                         them in order, loads of a step in front of its stores.
 //
-// Bound by memory (rows read and written once); the selection reads the weights from L1 after its first pass.
+// Bound by memory: rows read and written once.
 #include "mdb_common.cuh"
 
 namespace mdb {
 
-constexpr int kEvThreads = 1024, kEvPerThread = 8, kEvTile = kEvThreads * kEvPerThread;
+constexpr int kEvThreads = 1024, kEvQuads = 8, kEvStride = 4 * kEvThreads, kEvPage = kEvQuads * kEvStride;
 constexpr int kEvBins = 2048;
-constexpr int kEvMoveThreads = 256, kEvMoveRows = 8;       // pieces of 16 bytes in flight per thread
+constexpr int kEvMoveThreads = 256, kEvMoveRows = 256, kEvMovePieces = 8;      // rows of a CTA (or a step); pieces of 16 bytes in flight per thread
 
-// Bits that order like the numbers: negative ones upside down, -0 as 0, NaN lowest.
+__device__ __forceinline__ bool mdb_device_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Bits that order like the numbers: negative ones upside down, -0 as 0, NaN lowest; and the number back.
 __device__ __forceinline__ uint32_t ev_key(float w) {
-  if (w != w) return 0u;
   const uint32_t b = __float_as_uint(w + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t k = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+  return w != w ? 0u : k;
+}
+__device__ __forceinline__ float ev_number(uint32_t k) {
+  return __uint_as_float(k ^ (static_cast<uint32_t>(static_cast<int32_t>(~k) >> 31) | 0x80000000u));
 }
 
-// Exclusive sums over the CTA of two counts per thread, packed as 16 bits each (at most kEvTile each).
-__device__ __forceinline__ uint32_t ev_sums(uint32_t mine, uint32_t* warp_sums, uint32_t& all) {
+// Sum over the threads in front of this one, and of all, over the CTA.
+__device__ __forceinline__ uint32_t ev_before(uint32_t mine, uint32_t* warp_sums, uint32_t& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t upto = mine;
 #pragma unroll
@@ -38,24 +43,37 @@ __device__ __forceinline__ uint32_t ev_sums(uint32_t mine, uint32_t* warp_sums, 
   }
   if (lane == 31) warp_sums[warp] = upto;
   __syncthreads();
-  uint32_t w = warp_sums[lane], wu = w;                    // 32 warps
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, wu, o);
-    if (lane >= o) wu += up;
-  }
-  all = __shfl_sync(0xffffffffu, wu, 31);
-  const uint32_t before = __shfl_sync(0xffffffffu, wu - w, warp);
-  __syncthreads();
-  return before + upto - mine;
+  const uint32_t w = warp_sums[lane];                      // 32 warps
+  const uint32_t in_front = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u);
+  all = __reduce_add_sync(0xffffffffu, w);
+  return in_front + upto - mine;
 }
 
-__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const mdb_kv_evict_args a) {
+// Keys of weights [base, base + kEvPage) of the `front` ones, four neighbours at a time: k[4 q + c] is number base + q kEvStride + 4 tid
+// + c.  0, the lowest, behind the last: such a one counts among the lowest and lies behind all of them, so it never stays.
+__device__ __forceinline__ void ev_load(const float* w, int base, int front, bool wide, uint32_t (&k)[4 * kEvQuads]) {
+#pragma unroll
+  for (int q = 0; q < kEvQuads; ++q) {
+    if (base + q * kEvStride >= front) break;
+    const int i = base + q * kEvStride + 4 * static_cast<int>(threadIdx.x);
+    if (wide && i + 3 < front) {
+      const float4 v = *reinterpret_cast<const float4*>(w + i);
+      k[4 * q] = ev_key(v.x); k[4 * q + 1] = ev_key(v.y); k[4 * q + 2] = ev_key(v.z); k[4 * q + 3] = ev_key(v.w);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) k[4 * q + c] = i + c < front ? ev_key(w[i + c]) : 0u;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_kv_evict_args a) {
   __shared__ uint32_t counts[kEvBins];
-  __shared__ uint32_t warp_sums[32];
+  __shared__ uint32_t warp_sums[2][32];
+  __shared__ uint32_t quad_sums[kEvQuads * 32];
   __shared__ uint32_t found[2];
-  const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads, tid = threadIdx.x;
+  const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
+  for (int i = tid; i < kEvBins; i += kEvThreads) counts[i] = 0;
   pdl_wait();
   int n = a.seqlens[b];
   const int64_t most = min(static_cast<int64_t>(a.table_pages) * kPage, static_cast<int64_t>(a.weight_cols));
@@ -65,94 +83,118 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const mdb_kv_e
   }
   n = max(n, 0);
   const float* w = a.weights + b * a.weight_row + h * a.weight_head;
+  const bool wide = mdb_device_aligned16(w);
   int32_t* kept = a.kept + (static_cast<int64_t>(b) * a.kv_heads + h) * a.budget;
   float* w_out = a.weights_out == nullptr ? nullptr : a.weights_out + b * a.weight_out_row + h * a.weight_out_head;
-  const int stay = min(n, a.budget), recent = min(a.recent, stay);
-  const int front = n > a.budget ? n - recent : stay - recent;          // keys that are chosen from, and how many of them
-  const int need = stay - recent;
-  uint32_t last = 0, equals = 0;                           // key of the last one that stays; how many of its equals stay
-  if (need < front && need > 0) {
-    uint32_t prefix = 0, left = need;
+  // of n keys in front of the recent ones, `need` stay
+  const int recent = n > a.budget ? a.recent : n, front = n - recent, need = n > a.budget ? a.budget - recent : 0;
+  if (need > 0) {
+    uint32_t last = 0, left = need;                        // key of the last one that stays; how many of its equals do
+    uint32_t k[4 * kEvQuads];
+    ev_load(w, 0, front, wide, k);
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-      const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-      for (int i = tid; i < bins; i += kEvThreads) counts[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < front; i += kEvThreads) {
-        const uint32_t k = ev_key(w[i]);
-        if ((k & above) == prefix) atomicAdd(&counts[(k >> shift) & (bins - 1)], 1u);
+      constexpr int kShift[3] = {21, 10, 0};
+      const int shift = kShift[pass], bins = pass == 2 ? 1024 : 2048;
+      __syncthreads();                                     // the counts are zero
+      for (int base = 0; base < front; base += kEvPage) {
+        if (front > kEvPage && (base > 0 || pass > 0)) ev_load(w, base, front, wide, k);
+#pragma unroll
+        for (int q = 0; q < kEvQuads; ++q) {
+          if (base + q * kEvStride >= front) break;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t u = k[4 * q + c];
+            if (pass == 0 || (u ^ last) >> (pass == 1 ? 21 : 10) == 0) atomicAdd(&counts[(u >> shift) & (bins - 1)], 1u);
+          }
+        }
       }
       __syncthreads();
       // the bin, from the highest on, in which the left-th key lies: two bins per thread, highest first
       const int hi = bins - 1 - 2 * tid;
       const uint32_t c0 = hi >= 0 ? counts[hi] : 0u, c1 = hi >= 0 ? counts[hi - 1] : 0u;
-      uint32_t upto = c0 + c1;
-      const int lane = tid & 31, warp = tid >> 5;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += up;
-      }
-      if (lane == 31) warp_sums[warp] = upto;
-      __syncthreads();
-      uint32_t base = 0;
-      for (int i = 0; i < warp; ++i) base += warp_sums[i];
-      upto += base;
-      const uint32_t in_front = upto - c0 - c1;
-      if (in_front < left && left <= upto) {
+      if (hi >= 0) { counts[hi] = 0; counts[hi - 1] = 0; }
+      uint32_t all;
+      const uint32_t in_front = ev_before(c0 + c1, warp_sums[pass & 1], all);
+      if (in_front < left && left <= in_front + c0 + c1) {
         const bool second = left > in_front + c0;
         found[0] = static_cast<uint32_t>(second ? hi - 1 : hi);
         found[1] = left - in_front - (second ? c0 : 0u);
       }
       __syncthreads();
-      prefix |= found[0] << shift;
+      last |= found[0] << shift;
       left = found[1];
+    }
+    const uint32_t equals = left;
+    // places in order; all of a page is read before any of its places is written (weights_out may be weights)
+    uint32_t done = 0, done_equals = 0;
+    for (int base = 0; base < front; base += kEvPage) {
+      if (front > kEvPage) ev_load(w, base, front, wide, k);
+      uint32_t above = 0, same = 0, before[kEvQuads];      // a bit per key; counts in front within the warp: above | equals << 16
+#pragma unroll
+      for (int q = 0; q < kEvQuads; ++q) {
+        if (base + q * kEvStride >= front) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          above |= static_cast<uint32_t>(k[4 * q + c] > last) << (4 * q + c);
+          same |= static_cast<uint32_t>(k[4 * q + c] == last) << (4 * q + c);
+        }
+        const uint32_t mine = __popc(above >> (4 * q)) | __popc(same >> (4 * q)) << 16;
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += up;
+        }
+        before[q] = upto - mine;
+        if (lane == 31) quad_sums[q * 32 + warp] = upto;
+      }
+      __syncthreads();
+      // (a page has up to 2^15 of either kind: 16 bits each)
+      if (warp < kEvQuads && base + warp * kEvStride < front) {
+        const uint32_t mine = quad_sums[tid];
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += up;
+        }
+        quad_sums[tid] = upto - mine;
+        if (lane == 31) warp_sums[0][warp] = upto;
+      }
+      __syncthreads();
+      uint32_t page = 0;
+#pragma unroll
+      for (int q = 0; q < kEvQuads; ++q) {
+        if (base + q * kEvStride >= front) break;
+        const uint32_t in_front = page + quad_sums[q * 32 + warp] + before[q];
+        page += warp_sums[0][q];
+        uint32_t ties = done_equals + (in_front >> 16);
+        uint32_t at = done + (in_front & 0xffffu) + min(ties, equals);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const bool tie = same >> (4 * q + c) & 1;
+          if ((above >> (4 * q + c) & 1) || (tie && ties < equals)) {
+            kept[at] = base + q * kEvStride + 4 * tid + c;
+            if (w_out != nullptr) w_out[at] = ev_number(k[4 * q + c]);
+            ++at;
+          }
+          ties += tie;
+        }
+      }
+      done += page & 0xffffu;
+      done_equals += page >> 16;
       __syncthreads();
     }
-    last = prefix;
-    equals = left;
-  }
-  const bool all_stay = need == front;
-  // places in order; what a tile reads lies behind all that is written before it (weights_out may be weights)
-  uint32_t done = 0, done_equals = 0;
-  for (int base = 0; base < front && need > 0; base += kEvTile) {
-    float x[kEvPerThread];
-    uint32_t above = 0, same = 0, n_above = 0, n_same = 0;
-    const int i0 = base + tid * kEvPerThread;
-#pragma unroll
-    for (int i = 0; i < kEvPerThread; ++i) {
-      x[i] = i0 + i < front ? w[i0 + i] : 0.f;
-      const uint32_t k = ev_key(x[i]);
-      const bool there = i0 + i < front;
-      if (there && (all_stay || k > last)) { above |= 1u << i; ++n_above; }
-      else if (there && k == last) { same |= 1u << i; ++n_same; }
-    }
-    uint32_t all;
-    const uint32_t before = ev_sums(n_above | n_same << 16, warp_sums, all);
-    uint32_t ties = done_equals + (before >> 16);
-    uint32_t at = done + (before & 0xffffu) + min(ties, equals);
-#pragma unroll
-    for (int i = 0; i < kEvPerThread; ++i) {
-      const bool tie = same >> i & 1;
-      if ((above >> i & 1) || (tie && ties < equals)) {
-        kept[at] = i0 + i;
-        if (w_out != nullptr) w_out[at] = x[i];
-        ++at;
-      }
-      ties += tie;
-    }
-    done += all & 0xffffu;
-    done_equals += all >> 16;
-    __syncthreads();
   }
   for (int base = 0; base < a.budget - need; base += kEvThreads) {
     const int i = base + tid;
     const bool there = i < recent;
-    const float x = there && w_out != nullptr ? w[n - recent + i] : 0.f;
+    const float y = there && w_out != nullptr ? w[front + i] : 0.f;
     __syncthreads();
     if (i < a.budget - need) {
-      kept[need + i] = there ? n - recent + i : -1;
-      if (w_out != nullptr) w_out[need + i] = x;
+      kept[need + i] = there ? front + i : -1;
+      if (w_out != nullptr) w_out[need + i] = y;
     }
     __syncthreads();
   }
@@ -166,56 +208,62 @@ __device__ __forceinline__ int64_t ev_place(const int32_t* table, int pages, int
   return (static_cast<int64_t>(page) * kPage + i % kPage) * token_bytes;
 }
 
-// A CTA: `slice` pieces of 16 bytes of every row in [first, first + rows) of one (request, key head) of K or V.
+// `slice` pieces of 16 bytes of rows of one (request, key head) of K or V: of kEvMoveRows of them from kEvMoveRows blockIdx.y on, or
+// of all, kEvMoveRows at a time.
 template <bool IN_PLACE>
-__global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const mdb_kv_evict_args a, const int slice, const int rows_per_cta) {
+__global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const mdb_kv_evict_args a, const int slice) {
+  __shared__ int64_t places[2][kEvMoveRows];               // old and new byte offset of a row; old -1: stays
   pdl_launch_dependents();
-  pdl_wait();
-  const int pair = blockIdx.y >> 1, b = pair / a.kv_heads, h = pair % a.kv_heads, tid = threadIdx.x;
-  if (blockIdx.x == 0 && blockIdx.y == 2 * b * a.kv_heads && tid == 0) {
-    // (the lengths are read by the kernel in front alone, so that they may be replaced here)
-    const int64_t most = min(static_cast<int64_t>(a.table_pages) * kPage, static_cast<int64_t>(a.weight_cols));
-    a.seqlens_out[b] = max(0, static_cast<int>(min(static_cast<int64_t>(min(a.seqlens[b], a.budget)), most)));
-  }
-  unsigned char* cache = static_cast<unsigned char*>(blockIdx.y & 1 ? a.v_cache : a.k_cache);
+  const int pieces = a.row_bytes / 16, parts = pieces / slice;
+  int rest = blockIdx.x;
+  const int part = rest % parts; rest /= parts;
+  const bool values = rest & 1; rest >>= 1;
+  const int pair = rest, b = pair / a.kv_heads, h = pair % a.kv_heads, tid = threadIdx.x;
+  unsigned char* cache = static_cast<unsigned char*>(values ? a.v_cache : a.k_cache);
   const int32_t* kept = a.kept + static_cast<int64_t>(pair) * a.budget;
   const int32_t* from = a.block_table + static_cast<int64_t>(b) * a.table_stride;
   const int32_t* to = IN_PLACE ? from : a.out_table + static_cast<int64_t>(b) * a.out_table_stride;
   const int to_pages = IN_PLACE ? a.table_pages : a.out_table_pages;
   const int64_t token_bytes = static_cast<int64_t>(a.kv_heads) * a.row_bytes;
   const int piece = tid % slice, r0 = tid / slice, rows = kEvMoveThreads / slice;
-  const int64_t column = static_cast<int64_t>(h) * a.row_bytes + ((IN_PLACE ? blockIdx.x * slice : 0) + piece) * 16;
-  const int first = IN_PLACE ? 0 : blockIdx.x * rows_per_cta, end = IN_PLACE ? a.budget : min(a.budget, first + rows_per_cta);
+  cache += static_cast<int64_t>(h) * a.row_bytes + (part * slice + piece) * 16;
+  pdl_wait();
+  if (blockIdx.y == 0 && part == 0 && !values && h == 0 && tid == 0) {
+    // (the lengths are read by the kernel in front alone, so that they may be replaced here)
+    const int64_t most = min(static_cast<int64_t>(a.table_pages) * kPage, static_cast<int64_t>(a.weight_cols));
+    a.seqlens_out[b] = max(0, static_cast<int>(min(static_cast<int64_t>(min(a.seqlens[b], a.budget)), most)));
+  }
   bool bad = false;
-  const int pieces = a.row_bytes / 16;
-  // (to other pages a slice is a whole row, taken in several steps where it has more pieces than the CTA has threads)
-  for (int base = first; base < end; base += rows * kEvMoveRows) {
-    uint4 x[kEvMoveRows];
-    int64_t dst[kEvMoveRows];
-#pragma unroll
-    for (int j = 0; j < kEvMoveRows; ++j) {
-      const int i = base + j * rows + r0;
-      const int old = i < end ? kept[i] : -1;
-      dst[j] = -1;
+  for (int base = IN_PLACE ? 0 : blockIdx.y * kEvMoveRows; base < a.budget; base += kEvMoveRows) {
+    for (int r = tid; r < kEvMoveRows; r += kEvMoveThreads) {
+      const int i = base + r, old = i < a.budget ? kept[i] : -1;
+      int64_t src = -1, dst = -1;
       if (old >= 0 && !(IN_PLACE && old == i)) {
-        const int64_t src = ev_place(from, a.table_pages, a.num_pages, old, token_bytes);
-        const int64_t d = ev_place(to, to_pages, a.num_pages, i, token_bytes);
-        if (src >= 0 && d >= 0) {
-          dst[j] = d;
-          x[j] = *reinterpret_cast<const uint4*>(cache + src + column);
-          if (!IN_PLACE)
-            for (int p = piece + slice; p < pieces; p += slice)
-              *reinterpret_cast<uint4*>(cache + d + column + (p - piece) * 16) =
-                  *reinterpret_cast<const uint4*>(cache + src + column + (p - piece) * 16);
-        } else {
-          bad = true;
-        }
+        src = ev_place(from, a.table_pages, a.num_pages, old, token_bytes);
+        dst = ev_place(to, to_pages, a.num_pages, i, token_bytes);
+        if (src < 0 || dst < 0) { bad = true; src = -1; }
+      }
+      places[0][r] = src;
+      places[1][r] = dst;
+    }
+    __syncthreads();
+    for (int r = r0; r < kEvMoveRows; r += rows * kEvMovePieces) {
+      uint4 x[kEvMovePieces];
+#pragma unroll
+      for (int j = 0; j < kEvMovePieces; ++j) {
+        const int i = r + j * rows;
+        const int64_t src = i < kEvMoveRows ? places[0][i] : -1;
+        if (src >= 0) x[j] = *reinterpret_cast<const uint4*>(cache + src);
+      }
+      if (IN_PLACE) __syncthreads();                       // (every thread takes as many turns)
+#pragma unroll
+      for (int j = 0; j < kEvMovePieces; ++j) {
+        const int i = r + j * rows;
+        if (i < kEvMoveRows && places[0][i] >= 0) *reinterpret_cast<uint4*>(cache + places[1][i]) = x[j];
       }
     }
-    if (IN_PLACE) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kEvMoveRows; ++j)
-      if (dst[j] >= 0) *reinterpret_cast<uint4*>(cache + dst[j] + column) = x[j];
+    if (!IN_PLACE) break;
+    __syncthreads();
   }
   if (bad) report_status(MDB_STATUS_BAD_PAGE);
 }
@@ -234,22 +282,21 @@ extern "C" int mdb_kv_evict(const mdb_kv_evict_args* args, mdb_stream_t stream) 
   MDB_REQUIRE(a.k_cache && a.v_cache && a.weights && a.seqlens && a.seqlens_out && a.block_table && a.kept, MDB_ERR_ARG);
   MDB_REQUIRE(a.out_table == nullptr || (a.out_table_pages > 0 && (a.out_table_stride >= a.out_table_pages || a.bs <= 1)), MDB_ERR_ARG);
   MDB_REQUIRE(a.row_bytes % 16 == 0 && mdb_aligned16(a.k_cache) && mdb_aligned16(a.v_cache), MDB_ERR_ALIGN);
-  MDB_REQUIRE(static_cast<int64_t>(a.bs) * a.kv_heads <= 32767 && a.row_bytes <= 4096 && a.budget <= (1 << 29) && a.table_pages <= (1 << 22) && a.out_table_pages <= (1 << 22),
+  MDB_REQUIRE(static_cast<int64_t>(a.bs) * a.kv_heads <= 32767 && a.row_bytes <= 4096 && a.budget <= (1 << 23) && a.table_pages <= (1 << 22) && a.out_table_pages <= (1 << 22),
               MDB_ERR_UNSUPPORTED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int pairs = a.bs * a.kv_heads;
   int rc = mdb_launch(evict_select_kernel, dim3(pairs), dim3(kEvThreads), 0, st, a);
   if (rc != MDB_OK) return rc;
+  // slices of a power of two of pieces that divides the row, as wide as it goes; in place narrower, down to 32 bytes, until the
+  // SMs have two CTAs each
   const int pieces = a.row_bytes / 16;
+  int slice = 1;
+  while (slice < 32 && pieces % (2 * slice) == 0) slice *= 2;
   if (a.out_table == nullptr) {
-    // slices of at least 32 bytes, a power of two of pieces that divides the row, until the SMs have two CTAs each
-    int slice = 1;
-    while (slice < 32 && pieces % (2 * slice) == 0) slice *= 2;
     while (slice > 2 && static_cast<int64_t>(pairs) * 2 * (pieces / slice) < 2 * 148) slice /= 2;
-    return mdb_launch(evict_move_kernel<true>, dim3(pieces / slice, 2 * pairs), dim3(kEvMoveThreads), 0, st, a, slice, a.budget);
+    return mdb_launch(evict_move_kernel<true>, dim3(2 * pairs * (pieces / slice)), dim3(kEvMoveThreads), 0, st, a, slice);
   }
-  int slice = 1;                                           // the largest power of two of pieces in a row, up to a warp's worth
-  while (slice < 32 && 2 * slice <= pieces) slice *= 2;
-  const int rows = kEvMoveThreads / slice * kEvMoveRows;
-  return mdb_launch(evict_move_kernel<false>, dim3((a.budget + rows - 1) / rows, 2 * pairs), dim3(kEvMoveThreads), 0, st, a, slice, rows);
+  return mdb_launch(evict_move_kernel<false>, dim3(2 * pairs * (pieces / slice), (a.budget + kEvMoveRows - 1) / kEvMoveRows), dim3(kEvMoveThreads), 0, st, a,
+                    slice);
 }
