@@ -6,15 +6,14 @@
 // rot on pass.  Angles are products of 64 bits, taken to a fraction of a turn there: at position 131072 a product of 32 bits is
 // off by up to 2^-8 radian.  What is left is a number in [-1, 1] half turns, whose sine and cosine need no reduction.
 //
-// A CTA takes `tokens` tokens: sines and cosines of their pairs once, into shared memory, for all heads.  Threads lie in rows of
-// `width` (a power of two) along a head's pieces of 16 bytes, so that no index needs a division but a row's token.
-// It is bound by memory.  Measured: see the table of the cases; one token per CTA below 2 x 148 x 8 of them, four from there on.
+// A CTA takes some tokens: sines and cosines of their pairs once, into shared memory, for all heads.  A thread has one piece of 16 bytes
+// (half layout: two) of one head, whose place it works out once, and goes through the tokens with it, loads of kReBatch tokens in
+// front of their stores.  It is bound by memory.
 #include "mdb_common.cuh"
 
 namespace mdb {
 
-constexpr int kReThreads = 256;
-constexpr int kReManyTokens = 4;
+constexpr int kReThreads = 640, kReTokens = 16, kReBatch = 4;         // at most; tokens whose loads are in flight together
 
 template <typename T>
 struct ReVec;
@@ -50,94 +49,108 @@ __device__ __forceinline__ void re_store(bf16* p, float v) { *p = __float2bfloat
 
 // Pieces of a head: pairs of vectors (half layout) or vectors that hold whole pairs, then what passes.  WIDE: 16 bytes; otherwise
 // single numbers (sizes, strides or addresses that are no multiples of 16 bytes).
-template <typename T, bool WIDE, bool PAIRS>
-__global__ void __launch_bounds__(kReThreads) rotary_embed_kernel(const mdb_rotary_embed_args a, const int tokens, const int width) {
+template <typename T, bool WIDE, bool PAIRS, int BATCH>
+__global__ void __launch_bounds__(kReThreads, 2) rotary_embed_kernel(const mdb_rotary_embed_args a, const int tokens) {
   constexpr int V = WIDE ? ReVec<T>::kWide : 1;
   extern __shared__ float2 re_cs[];                        // [tokens][rot / 2]
+  __shared__ int64_t slots[kReTokens];                     // -1: skipped
   const int half = a.rot_dims / 2, tid = threadIdx.x;
   const int tok0 = blockIdx.x * tokens, count = min(tokens, a.n - tok0);
   pdl_launch_dependents();
+  // pieces of a head that turn, of one that turns or passes, of one that passes
+  const int turned = PAIRS ? (WIDE ? a.rot_dims / V : half) : half / V;
+  const int pieces = turned + (a.dim - a.rot_dims) / V, whole = a.dim / V;
+  const int turning = (a.heads + a.kv_heads) * pieces, columns = turning + (a.v != nullptr ? a.kv_heads * whole : 0);
   pdl_wait();
-  for (int i = tid; i < count * half; i += kReThreads) {
+  for (int i = tid; i < count * half; i += blockDim.x) {
     const int t = i / half, p = i - t * half;
     const double turns = static_cast<double>(a.positions[tok0 + t]) * (a.inv_freq[p] * 0.15915494309189533577);
     float s, c;
     sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
     re_cs[i] = make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
   }
+  if (a.slots != nullptr && tid < count) {
+    const int64_t slot = a.slots[tok0 + tid];
+    const bool there = slot >= 0 && slot < a.num_slots;
+    if (!there && slot != -1) report_status(MDB_STATUS_BAD_SLOT);
+    slots[tid] = there ? slot : -1;
+  }
   __syncthreads();
-
-  // pieces of a head that turn, and of one that turns or passes
-  const int turned = PAIRS ? (WIDE ? a.rot_dims / V : half) : half / V;
-  const int pieces = turned + (a.dim - a.rot_dims) / V;
-  const int heads = a.heads + a.kv_heads + (a.v != nullptr ? a.kv_heads : 0);
-  const float per_head = 1.0f / static_cast<float>(heads);
-  const int rows = kReThreads / width, u0 = tid & (width - 1);
-  for (int r = tid / width; r < count * heads; r += rows) {
-    const int t = static_cast<int>((static_cast<float>(r) + 0.5f) * per_head), head = r - t * heads;   // exact: r < 2^14
-    const int64_t row = tok0 + t;
-    const T* src;
-    T* dst;
-    int h = head;
-    bool turn = true;
-    if (head < a.heads) {
-      src = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
-      dst = static_cast<T*>(a.q_out) + row * a.q_out_row + h * a.q_out_head;
-    } else {
-      h = head - a.heads;
-      turn = h < a.kv_heads;
-      if (!turn) h -= a.kv_heads;
-      src = turn ? static_cast<const T*>(a.k) + row * a.k_row + h * a.k_head : static_cast<const T*>(a.v) + row * a.v_row + h * a.v_head;
-      if (a.slots != nullptr) {
-        const int64_t slot = a.slots[row];
-        if (slot < 0 || slot >= a.num_slots) {
-          if (slot != -1 && u0 == 0) report_status(MDB_STATUS_BAD_SLOT);
-          continue;
+  for (int column = tid; column < columns; column += blockDim.x) {
+    const bool value = column >= turning;
+    const int per = value ? whole : pieces, at = value ? column - turning : column;
+    int h = at / per, u = at - h * per;
+    const bool turn = !value && u < turned, query = !value && h < a.heads;
+    if (!value && !query) h -= a.heads;
+    // offset of the piece's first vector in a head
+    const int c = value ? u * V : turn ? (PAIRS && !WIDE ? 2 * u : u * V) : a.rot_dims + (u - turned) * V;
+    const int64_t from = query ? a.q_row : value ? a.v_row : a.k_row;
+    const T* src = static_cast<const T*>(query ? a.q : value ? a.v : a.k) + tok0 * from + h * (query ? a.q_head : value ? a.v_head : a.k_head) + c;
+    const bool stored = !query && a.slots != nullptr;
+    const int64_t to = stored ? static_cast<int64_t>(a.kv_heads) * a.dim : query ? a.q_out_row : a.k_out_row;
+    T* dst = static_cast<T*>(stored ? (value ? a.v_cache : a.k_cache) : query ? a.q_out : a.k_out) +
+             (stored ? h * a.dim : tok0 * to + h * (query ? a.q_out_head : a.k_out_head)) + c;
+    const float2* cs = re_cs + (PAIRS && WIDE ? u * V / 2 : u * V);
+    if (WIDE) {
+      for (int t0 = 0; t0 < count; t0 += BATCH) {
+        uint4 x[BATCH], y[PAIRS ? 1 : BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          if (t0 + j >= count) break;
+          x[j] = *reinterpret_cast<const uint4*>(src + (t0 + j) * from);
+          if (!PAIRS && turn) y[j] = *reinterpret_cast<const uint4*>(src + (t0 + j) * from + half);
         }
-        dst = static_cast<T*>(turn ? a.k_cache : a.v_cache) + (slot * a.kv_heads + h) * a.dim;
-      } else {
-        dst = static_cast<T*>(a.k_out) + row * a.k_out_row + h * a.k_out_head;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          if (t0 + j >= count) break;
+          const int64_t row = stored ? slots[t0 + j] : t0 + j;
+          if (row < 0) continue;
+          constexpr int W = ReVec<T>::kWide;
+          T* const d = dst + row * to;
+          const float2* const f = cs + (t0 + j) * half;
+          if (turn) {
+            float v[W];
+            ReVec<T>::unpack(x[j], v);
+            if (PAIRS) {
+#pragma unroll
+              for (int i = 0; i < W; i += 2) {
+                const float2 g = f[i / 2];
+                const float lo = v[i], hi = v[i + 1];
+                v[i] = lo * g.x - hi * g.y;
+                v[i + 1] = hi * g.x + lo * g.y;
+              }
+            } else {
+              float z[W];
+              ReVec<T>::unpack(y[PAIRS ? 0 : j], z);
+#pragma unroll
+              for (int i = 0; i < W; ++i) {
+                const float2 g = f[i];
+                const float lo = v[i], hi = z[i];
+                v[i] = lo * g.x - hi * g.y;
+                z[i] = hi * g.x + lo * g.y;
+              }
+              *reinterpret_cast<uint4*>(d + half) = ReVec<T>::pack(z);
+            }
+            x[j] = ReVec<T>::pack(v);
+          }
+          *reinterpret_cast<uint4*>(d) = x[j];
+        }
       }
-    }
-    const float2* cs = re_cs + t * half;
-    const int end = turn ? pieces : a.dim / V;
-    for (int u = u0; u < end; u += width) {
-      if (!turn || u >= turned) {
-        const int c = turn ? a.rot_dims + (u - turned) * V : u * V;
-        if (WIDE) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-        else dst[c] = src[c];
-      } else if (WIDE && PAIRS) {
-        constexpr int W = ReVec<T>::kWide;
-        float x[W];
-        ReVec<T>::unpack(*reinterpret_cast<const uint4*>(src + u * V), x);
-#pragma unroll
-        for (int i = 0; i < W; i += 2) {
-          const float2 f = cs[(u * V + i) / 2];
-          const float lo = x[i], hi = x[i + 1];
-          x[i] = lo * f.x - hi * f.y;
-          x[i + 1] = hi * f.x + lo * f.y;
+    } else {
+      for (int t = 0; t < count; ++t) {
+        const int64_t row = stored ? slots[t] : t;
+        if (row < 0) continue;
+        const T* const x = src + t * from;
+        T* const d = dst + row * to;
+        if (turn) {
+          const int other = PAIRS ? 1 : half;
+          const float2 g = cs[t * half];
+          const float lo = re_load(x), hi = re_load(x + other);
+          re_store(d, lo * g.x - hi * g.y);
+          re_store(d + other, hi * g.x + lo * g.y);
+        } else {
+          d[0] = x[0];
         }
-        *reinterpret_cast<uint4*>(dst + u * V) = ReVec<T>::pack(x);
-      } else if (WIDE) {
-        constexpr int W = ReVec<T>::kWide;
-        float x[W], y[W];
-        ReVec<T>::unpack(*reinterpret_cast<const uint4*>(src + u * V), x);
-        ReVec<T>::unpack(*reinterpret_cast<const uint4*>(src + half + u * V), y);
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float2 f = cs[u * V + i];
-          const float lo = x[i], hi = y[i];
-          x[i] = lo * f.x - hi * f.y;
-          y[i] = hi * f.x + lo * f.y;
-        }
-        *reinterpret_cast<uint4*>(dst + u * V) = ReVec<T>::pack(x);
-        *reinterpret_cast<uint4*>(dst + half + u * V) = ReVec<T>::pack(y);
-      } else {
-        const int c0 = PAIRS ? 2 * u : u, c1 = PAIRS ? 2 * u + 1 : u + half;
-        const float2 f = cs[u];
-        const float lo = re_load(src + c0), hi = re_load(src + c1);
-        re_store(dst + c0, lo * f.x - hi * f.y);
-        re_store(dst + c1, hi * f.x + lo * f.y);
       }
     }
   }
@@ -152,16 +165,19 @@ static int re_launch(const mdb_rotary_embed_args& a, cudaStream_t st) {
                     even(a.k_out, a.k_out_row, a.k_out_head) && even(a.k_cache, 0, 0) && even(a.v_cache, 0, 0);
   const int v = wide ? W : 1;
   const int pieces = (a.interleaved && wide ? a.rot_dims / v : a.rot_dims / 2 / v) + (a.dim - a.rot_dims) / v;
-  int width = 1;
-  while (width < pieces && width < kReThreads) width *= 2;
-  const int tokens = a.n >= 2 * 148 * 8 ? kReManyTokens : 1;
-  const dim3 grid((a.n + tokens - 1) / tokens), block(kReThreads);
+  const int columns = (a.heads + a.kv_heads) * pieces + (a.v != nullptr ? a.kv_heads * (a.dim / v) : 0);
+  // turns of about as many columns each, whole warps
+  const int turns = (columns + kReThreads - 1) / kReThreads, threads = ((columns + turns - 1) / turns + 31) / 32 * 32;
+  // a token per CTA while all CTAs are resident at once (48 registers a thread), then as few full rounds as there can be
+  const int64_t resident = 148 * (65536 / (48 * threads)), rounds = (a.n + resident * kReTokens - 1) / (resident * kReTokens);
+  int tokens = static_cast<int>((a.n + resident * rounds - 1) / (resident * rounds));
+  while (tokens > 1 && sizeof(float2) * tokens * (a.rot_dims / 2) > 40 * 1024) tokens /= 2;
+  const dim3 grid((a.n + tokens - 1) / tokens), block(threads);
   const size_t smem = sizeof(float2) * tokens * (a.rot_dims / 2);
-  if (wide)
-    return a.interleaved ? mdb_launch(rotary_embed_kernel<T, true, true>, grid, block, smem, st, a, tokens, width)
-                         : mdb_launch(rotary_embed_kernel<T, true, false>, grid, block, smem, st, a, tokens, width);
-  return a.interleaved ? mdb_launch(rotary_embed_kernel<T, false, true>, grid, block, smem, st, a, tokens, width)
-                       : mdb_launch(rotary_embed_kernel<T, false, false>, grid, block, smem, st, a, tokens, width);
+  const auto go = [&](auto kernel) { return mdb_launch(kernel, grid, block, smem, st, a, tokens); };
+  if (!wide) return a.interleaved ? go(rotary_embed_kernel<T, false, true, 1>) : go(rotary_embed_kernel<T, false, false, 1>);
+  if (tokens == 1) return a.interleaved ? go(rotary_embed_kernel<T, true, true, 1>) : go(rotary_embed_kernel<T, true, false, 1>);
+  return a.interleaved ? go(rotary_embed_kernel<T, true, true, kReBatch>) : go(rotary_embed_kernel<T, true, false, kReBatch / 2>);
 }
 
 }  // namespace mdb
@@ -178,7 +194,6 @@ extern "C" int mdb_rotary_embed(const mdb_rotary_embed_args* args, mdb_stream_t 
   MDB_REQUIRE(a.q && a.q_out && a.positions && (a.rot_dims == 0 || a.inv_freq), MDB_ERR_ARG);
   if (a.slots != nullptr) MDB_REQUIRE(a.kv_heads > 0 && a.k && a.k_cache && (!a.v || a.v_cache) && a.num_slots > 0, MDB_ERR_ARG);
   else MDB_REQUIRE((a.kv_heads == 0 || (a.k && a.k_out)) && a.v == nullptr, MDB_ERR_ARG);
-  // a row's index has to be exact in the kernel's fp32 division, and the sines of four tokens to fit 48 KB
-  MDB_REQUIRE(a.dim <= 1024 && static_cast<int64_t>(a.heads) + 2 * static_cast<int64_t>(a.kv_heads) <= 2048, MDB_ERR_UNSUPPORTED);
+  MDB_REQUIRE(a.dim <= 1024 && static_cast<int64_t>(a.heads) + 2 * static_cast<int64_t>(a.kv_heads) <= 65536, MDB_ERR_UNSUPPORTED);
   return a.dtype == MDB_BF16 ? re_launch<bf16>(a, static_cast<cudaStream_t>(stream)) : re_launch<float>(a, static_cast<cudaStream_t>(stream));
 }
