@@ -13,8 +13,8 @@
 // a unit leaves its sums (max, sum, O: fp32) at the rows' place, a part that goes on with one at its CTA's place (a CTA has one
 // such part at most: its first); info[unit] says how many CTAs follow.
 //
-// Roles: a TMA warp (query tiles, rings of K and V tiles), an MMA warp, two groups of four softmax warps, a row per thread.  Units of
-// two tiles take both groups; units of one take them in turn, each with the query tile, the output columns and the barriers of its
+// Roles: a warp that works out the CTA's parts and hands them on through shared memory, a TMA warp (query tiles, rings of K and V
+// tiles), an MMA warp, two groups of four softmax warps, a row per thread.  Units of two tiles take both groups; units of one take them in turn, each with the query tile, the output columns and the barriers of its
 // group, so that one's start lies under the other's end.
 // Tensor memory: S_0 (P_0) | S_1 (P_1) | O_0 | O_1, 128 columns each.  Of two tiles each has its score columns, of one it takes both in
 // turn, the next scores ahead of P V.  P goes back into the columns its scores came from, in two halves, of which the first is
@@ -25,18 +25,20 @@
 namespace mdb {
 
 // Times: a key tile of one query tile, of two, start and end of a unit; the least share of a CTA.
-constexpr uint32_t kShOneStep = 6, kShTwoStep = 8, kShUnit = 10, kShMinShare = 16;
+constexpr uint32_t kShOneStep = 5, kShTwoStep = 8, kShUnit = 6, kShMinShare = 16;
 
 struct ShPlan {
   static constexpr int kKStages = 3, kVStages = 2;
   static constexpr int kQBytes = 2 * 128 * 128;            // a tile: two channel halves of [128 rows][128 B]
-  static constexpr int kThreads = 384;                     // eight softmax warps, TMA, MMA; two idle
-  static constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
+  static constexpr int kThreads = 384;                     // eight softmax warps, TMA, MMA, parts; one idle
+  static constexpr int kParts = 4;                         // handed on ahead
+  static constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;       // (216 and 72: 331 for 321 us, 64 blocks of 32 behind 16384 keys)
   static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "registers after the split");
   static constexpr int kOffK = 2 * kQBytes;
   static constexpr int kOffV = kOffK + kKStages * kAtTileBytes;
   static constexpr int kOffBars = kOffV + kVStages * kAtTileBytes;
-  static constexpr int kSmemBytes = 1024 + kOffBars + 512;
+  static constexpr int kOffParts = kOffBars + 384, kPartBytes = 48;
+  static constexpr int kSmemBytes = 1024 + kOffParts + kParts * kPartBytes;
 };
 static_assert(ShPlan::kSmemBytes <= 227 * 1024, "shared memory of the shared-prefix attention");
 
@@ -64,7 +66,8 @@ struct ShArgs {
 // of a group x: Q, O and P V barriers; S and P barriers by group and score columns
 enum {
   kShBarQFull = 0, kShBarQEmpty = 2, kShBarKFull = 4, kShBarKEmpty = 7, kShBarVFull = 10, kShBarVEmpty = 12, kShBarSFull = 14 /* 2 x + buf */,
-  kShBarPDone = 18, kShBarOFull = 20, kShBarOEmpty = 22, kShBarPFull = 24 /* 2 (2 x + buf) + half */, kShBarCount = 32
+  kShBarPDone = 18, kShBarOFull = 20, kShBarOEmpty = 22, kShBarPFull = 24 /* 2 (2 x + buf) + half */, kShBarPartFull = 32,
+  kShBarPartEmpty = 36, kShBarCount = 40
 };
 
 __device__ __forceinline__ int sh_prefix(const ShArgs& a) {
@@ -83,17 +86,18 @@ __device__ __forceinline__ uint32_t sh_cut(uint32_t x, uint32_t steps, int per) 
 }
 
 // A part of a unit.
-struct ShPart {
+struct __align__(16) ShPart {
   int req;                 // -1: the prefix
-  int kvh, unit;           // unit: its place in info
-  int tok0;                // first token of the first tile (of all requests' tokens)
-  bool two;                // there is a second tile
+  int kvh, tok0;           // first token of the first tile (of all requests' tokens)
+  int two;                 // there is a second tile
   int slot;                // group of a unit of one tile
   int tok_end, box;        // the rows end here; tokens of a tile
-  int len, k0, k1;         // keys of the unit; key tiles of the part
+  int len, k0, k1;         // keys of the unit; key tiles of the part (k1 0: there are no more parts)
+  int unit, followers;     // place in info; CTAs behind this one that have a part of the unit
 };
+static_assert(sizeof(ShPart) == ShPlan::kPartBytes, "a part's size");
 
-// A CTA's run of the list; every role walks it the same way.
+// A CTA's run of the list.
 struct ShWalk {
   uint32_t x0, x1, at;           // run, start of the unit at the cursor
   uint32_t per, rest, share;     // length of the list = per * share + rest, over so many CTAs
@@ -174,30 +178,38 @@ struct ShWalk {
       p.tok_end = prefix ? a.tokens : (b + 1) * a.block;
       p.two = tiles == 2 && p.tok0 + p.box < p.tok_end;
       p.len = n;
+      const uint32_t s = at;
       at += cost;
       if (++u == units) { u = 0; ++kvh; }
       if (p.k1 > p.k0) {
         p.slot = turn;
         if (!p.two) turn ^= 1;
+        p.followers = 0;
+        if (x1 < at)
+          for (uint32_t c = blockIdx.x + 1; c < share; ++c, ++p.followers) {
+            const uint32_t x = start_of(c);
+            if (x >= at || sh_cut(x - s, steps, tiles) >= steps) break;
+          }
         return true;
       }
     }
     return false;
   }
-  // how many CTAs behind this one have a part of the unit that `next` gave last
-  __device__ __forceinline__ int followers(const ShArgs& a, const ShPart& p) const {
-    const uint32_t steps = sh_steps(p.len);
-    const int tiles = p.req < 0 ? a.per_p : a.per_o;
-    const uint32_t s = at - sh_cost(steps, tiles);
-    int n = 0;
-    for (uint32_t c = blockIdx.x + 1; c < share; ++c, ++n) {
-      const uint32_t x = start_of(c);
-      if (x >= at || sh_cut(x - s, steps, tiles) >= steps) break;
-    }
-    return n;
-  }
 };
 
+// The same number to one, eight or 32 columns of every lane.
+__device__ __forceinline__ void tmem_fill1(uint32_t taddr, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void tmem_fill8(uint32_t taddr, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(taddr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void tmem_fill32(uint32_t taddr, float v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, "
+      "%1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(taddr), "f"(v)
+      : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -208,7 +220,7 @@ __global__ void __launch_bounds__(ShPlan::kThreads, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_constant__ CUtensorMap map_qo, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const ShArgs a) {
   using P = ShPlan;
-  constexpr int kProducerWarp = 8, kMmaWarp = 9;
+  constexpr int kProducerWarp = 8, kMmaWarp = 9, kPartsWarp = 10;
   extern __shared__ __align__(1024) unsigned char sh_smem_raw[];
   const uint32_t raw = smem_u32(sh_smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gen_base = sh_smem_raw + (base - raw);
@@ -219,7 +231,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
 
   pdl_launch_dependents();
   if (warp == 0) {
-    mbar_init(bar(lane), lane >= kShBarOEmpty ? 4 : 1);      // (those of the softmax warps are the last ones)
+    mbar_init(bar(lane), lane >= kShBarOEmpty ? 4 : 1);      // (the softmax warps' are the last ones of these)
+    if (lane < kShBarCount - 32) mbar_init(bar(32 + lane), 32 + lane >= kShBarPartEmpty ? 10 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -232,9 +245,25 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = misc[0];
   pdl_wait();
-  ShWalk walk;
-  walk.start(a);
+  ShPart* const parts = reinterpret_cast<ShPart*>(gen_base + P::kOffParts);
   ShPart w;
+  AtRing part;
+  // The next part (false: none, or `ok` is), by a warp or by its first thread.
+  auto take = [&](bool& ok, uint32_t threads = 0xffffffffu) {
+    ok = mbar_wait(bar(kShBarPartFull + part.stage), part.phase);
+    ok = __all_sync(threads, ok);
+    if (!ok) return false;
+    const int4* from = reinterpret_cast<const int4*>(parts + part.stage);
+    const int4 p0 = from[0], p1 = from[1];
+    const int2 p2 = *reinterpret_cast<const int2*>(from + 2);
+    w.req = p0.x; w.kvh = p0.y; w.tok0 = p0.z; w.two = p0.w;
+    w.slot = p1.x; w.tok_end = p1.y; w.box = p1.z; w.len = p1.w;
+    w.k0 = p2.x; w.k1 = p2.y;
+    __syncwarp(threads);
+    if (lane == 0) mbar_arrive(bar(kShBarPartEmpty + part.stage));
+    part.advance(P::kParts);
+    return w.k1 > 0;
+  };
 
   if (warp >= kProducerWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kOtherRegs));
@@ -257,11 +286,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
           r.advance(stages);
           return true;
         };
-        if (blockIdx.x == 0 && a.prefix_len != nullptr && *a.prefix_len > walk.plen) report_status(MDB_STATUS_BAD_PAGE);
-        while (ok && walk.next(a, w)) {
+        while (take(ok, 1u)) {
           const int32_t* table = w.req < 0 ? a.prefix_table : a.block_table + static_cast<int64_t>(w.req) * a.table_stride;
           int page = table[w.k0 * kAtKeys / kPage];
-          if (w.req >= 0 && w.k0 == 0 && a.ctx_lens[w.req] > w.len) report_status(MDB_STATUS_BAD_PAGE);
           const CUtensorMap* map_q = w.req < 0 ? &map_qp : &map_qo;
           for (int x = w.two ? 0 : w.slot; x <= (w.two ? 1 : w.slot); ++x) {
             if (!mbar_wait(bar(kShBarQEmpty + x), (q_phase >> x & 1) ^ 1)) { ok = false; break; }
@@ -284,6 +311,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
             ok = load_tile(&map_k, base + P::kOffK, kShBarKFull, kShBarKEmpty, P::kKStages, kr, pend_k, par_k, w.kvh, row) &&
                  load_tile(&map_v, base + P::kOffV, kShBarVFull, kShBarVEmpty, P::kVStages, vr, pend_v, par_v, w.kvh, row);
           }
+          if (!ok) break;
         }
         if (!ok) {
           report_status(MDB_STATUS_WAIT_TIMEOUT);
@@ -301,7 +329,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
       AtRing kr, vr;
       uint32_t p_phase = 0 /* bit 2 x + buf */, o_phase = 0, q_phase = 0 /* bit x */;
       int buf = 0;                         // score columns of the next tile of a unit of one
-      bool ok = true, have = walk.next(a, w), ahead = false;
+      bool ok = true, have = take(ok), ahead = false;
       auto wait_q = [&](int x) {
         const bool r = mbar_wait_w(bar(kShBarQFull + x), q_phase >> x & 1);
         q_phase ^= 1u << x;
@@ -370,7 +398,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
               if (j + 2 == w.k1) { umma_commit_w(bar(kShBarQEmpty)); umma_commit_w(bar(kShBarQEmpty + 1)); }
             }
           }
-          have = ok && walk.next(a, w);
+          have = ok && take(ok);
         } else {
           const int x = w.slot, k0 = w.k0, k1 = w.k1;
           if (!ahead) {
@@ -390,7 +418,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
               release_k();
               if (j + 2 == k1) umma_commit_w(bar(kShBarQEmpty + x));
             } else {
-              have = walk.next(a, w);
+              have = take(ok);
+              if (!ok) break;
               if (have && !w.two) {
                 ok = wait_q(w.slot) && wait_k();
                 if (!ok) break;
@@ -409,6 +438,25 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
         }
       }
       if (!ok && lane == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
+    } else if (warp == kPartsWarp) {
+      // ----------------------------------------------------------------- the CTA's parts
+      ShWalk walk;
+      walk.start(a);
+      if (lane == 0) {
+        if (blockIdx.x == 0 && a.prefix_len != nullptr && *a.prefix_len > walk.plen) report_status(MDB_STATUS_BAD_PAGE);
+        for (bool more = true; more;) {
+          more = walk.next(a, w);
+          if (!more) w.k1 = 0;
+          if (!mbar_wait(bar(kShBarPartEmpty + part.stage), part.phase ^ 1)) { report_status(MDB_STATUS_WAIT_TIMEOUT); break; }
+          parts[part.stage] = w;
+          mbar_arrive(bar(kShBarPartFull + part.stage));
+          part.advance(P::kParts);
+          if (more && w.k0 == 0) {
+            a.info[w.unit] = make_int2(static_cast<int>(blockIdx.x), w.followers);
+            if (w.req >= 0 && a.ctx_lens[w.req] > w.len) report_status(MDB_STATUS_BAD_PAGE);
+          }
+        }
+      }
     }
   } else {
     // ------------------------------------------------------------------- softmax
@@ -423,10 +471,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
     int buf0 = 0;                       // score columns of its first tile, in a unit of one
     uint32_t s_phase = 0 /* bit per score columns */, o_phase = 0, done_phase = 0;      // done: of the last P V
     bool ok = true;
-    while (ok && walk.next(a, w)) {
+    while (take(ok)) {
       const int tiles = w.k1 - w.k0;
       const bool mine = w.two || w.slot == x;
-      if (row == 0 && w.k0 == 0 && (w.two ? x == 0 : mine)) a.info[w.unit] = make_int2(static_cast<int>(blockIdx.x), walk.followers(a, w));
       if (mine) {
         const int tok = w.tok0 + (w.two ? x * w.box : 0) + tok_local;
         const bool row_valid = tok_local < w.box && tok < w.tok_end;
@@ -453,6 +500,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_row + (c >> 3) * kAtHalfBytes + (c & 7) * 16), "r"(0u) : "memory");
             }
             fence_async_smem();
+            // and their scores (NaN among them) are minus infinity: in place, where a few instructions do
+            int c = nv;
+            for (; c & 7; ++c) tmem_fill1(s_addr + c, -INFINITY);
+            for (; c & 31; c += 8) tmem_fill8(s_addr + c, -INFINITY);
+            for (; c < kAtKeys; c += 32) tmem_fill32(s_addr + c, -INFINITY);
+            tmem_st_wait();
           }
           const uint32_t p_full = bar(kShBarPFull + 2 * (2 * x + buf));
           if (warp_valid) {
@@ -460,10 +513,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
             tmem_ld_wait();
-            if (nv < kAtKeys) {
-#pragma unroll
-              for (int c = 0; c < kAtKeys; ++c) if (c >= nv) s[c] = -INFINITY;   // also replaces NaN from stale rows
-            }
             float mxv[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) mxv[k] = fmaxf(s[k], s[4 + k]);
