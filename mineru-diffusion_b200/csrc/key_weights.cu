@@ -5,12 +5,12 @@
 //
 // lse is what the attention over all the keys returned (attention_shared.cu), so one pass over the keys is enough and no other
 // statistic is needed.  The product is formed the other way round than in the attention kernels: the 128 keys of a tile are
-// the rows (A operand, one key per tensor-memory lane) and the queries the columns (N = 16 .. 256), so that the sum over queries
+// the rows (A operand, one key per tensor-memory lane) and the queries the columns (N = 16 .. 128), so that the sum over queries
 // is a sum over one thread's registers: no exchange between threads, no atomics, one fixed order.
 //
 // The key tiles of all requests and heads are one list, of which every CTA takes an equal run (lengths differ and are known to
-// the device alone).  Roles: a TMA warp (query tile of the run's request and head, ring of key tiles), an MMA warp, and two
-// groups of four warps that take every other tile.  More than 256 rows per key head go in blocks of rows over up to 16 tiles at
+// the device alone).  Roles: a TMA warp (query tile of the run's request and head, ring of key tiles), an MMA warp, and four
+// groups of four warps that take the tiles in turn.  More than 128 rows per key head go in blocks of rows over up to 16 tiles at
 // a time, sums in shared memory.
 //
 // Bound by memory (256 bytes per key and head) up to 128 rows, beyond that by the exponentials: 16 a clock and SM.
@@ -18,8 +18,8 @@
 
 namespace mdb {
 
-constexpr int kKwThreads = 320;                            // two groups of four warps, TMA, MMA
-constexpr int kKwMaxRows = 256;                            // rows of a block = the widest N
+constexpr int kKwGroups = 4, kKwThreads = 128 * kKwGroups + 64;       // groups of four warps; TMA, MMA
+constexpr int kKwMaxRows = 512 / kKwGroups;                // rows of a block: the groups' scores fill tensor memory
 constexpr int kKwSegTiles = 16;                            // tiles walked at a time where there are several blocks of rows
 constexpr int kKwMaxStages = 6;
 constexpr int kKwSmem = 226 * 1024;
@@ -33,7 +33,7 @@ struct KwArgs {
   int bs, block, hq, hkv, group, table_stride, table_pages, num_pages;
   int64_t cols;                // of out and previous
   int tokens, row_blocks;      // of a block of rows
-  int n_pad, q_bufs, stages;
+  int n_pad, stages;
   float scale_log2, decay;
 };
 
@@ -108,7 +108,10 @@ struct KwWalk {
 };
 
 // barrier slots
-enum { kKwBarQFull = 0, kKwBarQEmpty = 2, kKwBarSFull = 4, kKwBarSEmpty = 6, kKwBarKFull = 8, kKwBarKEmpty = 8 + kKwMaxStages, kKwBarCount = 8 + 2 * kKwMaxStages };
+enum {
+  kKwBarQFull = 0, kKwBarQEmpty = 2, kKwBarSFull = 4, kKwBarSEmpty = kKwBarSFull + kKwGroups, kKwBarKFull = kKwBarSEmpty + kKwGroups,
+  kKwBarKEmpty = kKwBarKFull + kKwMaxStages, kKwBarCount = kKwBarKEmpty + kKwMaxStages
+};
 
 __global__ void __launch_bounds__(kKwThreads, 1)
 key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const KwArgs a) {
@@ -116,17 +119,17 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const uint32_t raw = smem_u32(kw_smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gen_base = kw_smem_raw + (base - raw);
   const int q_bytes = a.n_pad * 256;                       // two channel halves of [n_pad][128 B]
-  const uint32_t off_k = a.q_bufs * q_bytes, off_lse = off_k + a.stages * kAtTileBytes, off_sums = off_lse + 8 * kKwMaxRows * 4;
+  const uint32_t off_k = 2 * q_bytes, off_lse = off_k + a.stages * kAtTileBytes, off_sums = off_lse + 4 * kKwGroups * kKwMaxRows * 4;
   const uint32_t off_bars = off_sums + (a.row_blocks > 1 ? kKwSegTiles * kAtKeys * 4 : 0);
   const uint32_t bars = base + off_bars;
   auto bar = [&](int slot) { return bars + 8u * static_cast<uint32_t>(slot); };
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gen_base + off_bars + 8 * kKwBarCount);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kProducerWarp = 8, kMmaWarp = 9;
+  constexpr int kProducerWarp = 4 * kKwGroups, kMmaWarp = kProducerWarp + 1;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kKwBarCount; ++s) mbar_init(bar(s), s >= kKwBarSEmpty && s < kKwBarSEmpty + 2 ? 4 : 1);
+    for (int s = 0; s < kKwBarCount; ++s) mbar_init(bar(s), s >= kKwBarSEmpty && s < kKwBarSEmpty + kKwGroups ? 4 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -158,7 +161,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           tma_load_3d(q_tile + a.n_pad * 128, &map_q, 64, s.h * a.group, s.b * a.block + rb * a.tokens, qf);
           pend_q |= 1u << qr.stage;
           par_q = (par_q & ~(1u << qr.stage)) | (qr.phase << qr.stage);
-          qr.advance(a.q_bufs);
+          qr.advance(2);
           for (int j = 0; j < s.tiles; ++j) {
             const int key0 = (s.tile + j) * kAtKeys;
             int page = a.block_table[static_cast<int64_t>(s.b) * a.table_stride + key0 / kPage];
@@ -180,7 +183,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       if (!ok) {
         report_status(MDB_STATUS_WAIT_TIMEOUT);
         for (int i = 0; i < a.stages; ++i) if (pend_k >> i & 1) mbar_wait(bar(kKwBarKFull + i), par_k >> i & 1);
-        for (int i = 0; i < a.q_bufs; ++i) if (pend_q >> i & 1) mbar_wait(bar(kKwBarQFull + i), par_q >> i & 1);
+        for (int i = 0; i < 2; ++i) if (pend_q >> i & 1) mbar_wait(bar(kKwBarQFull + i), par_q >> i & 1);
       }
     }
   } else if (warp == kMmaWarp) {
@@ -194,21 +197,21 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (!mbar_wait_w(bar(kKwBarQFull + qr.stage), qr.phase)) { ok = false; break; }
         const uint32_t q_tile = base + qr.stage * q_bytes;
         for (int j = 0; j < s.tiles; ++j) {
-          const int buf = (seg_base + j) & 1;
+          const int buf = (seg_base + j) % kKwGroups;
           if (!mbar_wait_w(bar(kKwBarKFull + kr.stage), kr.phase) || !mbar_wait_w(bar(kKwBarSEmpty + buf), (s_phase >> buf & 1) ^ 1)) { ok = false; break; }
           s_phase ^= 1u << buf;
           tc_fence_after();
           const uint32_t k_tile = base + off_k + kr.stage * kAtTileBytes;
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_bf16_w(tmem_base + buf * 256, umma_desc_sw128(k_tile + (kk >> 2) * kAtHalfBytes) + 2 * (kk & 3),
+            umma_bf16_w(tmem_base + buf * kKwMaxRows, umma_desc_sw128(k_tile + (kk >> 2) * kAtHalfBytes) + 2 * (kk & 3),
                         umma_desc_sw128(q_tile + (kk >> 2) * (a.n_pad * 128)) + 2 * (kk & 3), idesc, kk > 0 ? 1u : 0u);
           umma_commit_w(bar(kKwBarKEmpty + kr.stage));
           umma_commit_w(bar(kKwBarSFull + buf));
           kr.advance(a.stages);
         }
         umma_commit_w(bar(kKwBarQEmpty + qr.stage));
-        qr.advance(a.q_bufs);
+        qr.advance(2);
       }
       seg_base += s.tiles;
     }
@@ -222,7 +225,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     // behind the last tile of every request: no key, no weight
     for (int64_t r = blockIdx.x; r < static_cast<int64_t>(a.bs) * a.hkv; r += gridDim.x) {
       const int tiles = (kw_len(a, static_cast<int>(r / a.hkv)) + kAtKeys - 1) / kAtKeys;
-      for (int64_t i = static_cast<int64_t>(tiles) * kAtKeys + threadIdx.x; i < a.cols; i += 256) a.out[r * a.cols + i] = 0.f;
+      for (int64_t i = static_cast<int64_t>(tiles) * kAtKeys + threadIdx.x; i < a.cols; i += 128 * kKwGroups) a.out[r * a.cols + i] = 0.f;
     }
     uint32_t s_phase = 0, seg_base = 0;
     bool ok = true;
@@ -238,7 +241,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         __syncwarp();
         for (int j = 0; j < s.tiles; ++j) {
-          if (((seg_base + j) & 1) != wg) continue;
+          if (static_cast<int>((seg_base + j) % kKwGroups) != wg) continue;
           const int key = (s.tile + j) * kAtKeys + tid;
           const bool last_block = rb == a.row_blocks - 1;
           const float before = last_block && a.previous != nullptr && key < s.len ? a.previous[row + key] * a.decay : 0.f;
@@ -250,7 +253,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           f32x2 part[4] = {0ull, 0ull, 0ull, 0ull};
           for (int c = 0; c < rows; c += 32) {
             float x[32];
-            tmem_ld32(tmem_base + wg * 256 + lane_field + c, x);      // (columns behind the last row are not looked at)
+            tmem_ld32(tmem_base + wg * kKwMaxRows + lane_field + c, x);      // (columns behind the last row are not looked at)
             tmem_ld_wait();
             if (c + 32 <= rows) {
 #pragma unroll
@@ -340,11 +343,10 @@ extern "C" int mdb_key_weights(const mdb_key_weights_args* args, mdb_stream_t st
   a.tokens = w.block < kKwMaxRows / group ? w.block : kKwMaxRows / group;
   a.row_blocks = (w.block + a.tokens - 1) / a.tokens;
   a.n_pad = (a.tokens * group + 15) / 16 * 16;
-  a.q_bufs = a.n_pad > 128 && a.row_blocks == 1 ? 1 : 2;        // (room for key tiles; the rows change once in a run)
-  const int rest = 1024 + 8 * kKwMaxRows * 4 + (a.row_blocks > 1 ? kKwSegTiles * kAtKeys * 4 : 0) + 8 * kKwBarCount + 16;
-  a.stages = (kKwSmem - rest - a.q_bufs * a.n_pad * 256) / kAtTileBytes;
+  const int rest = 1024 + 4 * kKwGroups * kKwMaxRows * 4 + (a.row_blocks > 1 ? kKwSegTiles * kAtKeys * 4 : 0) + 8 * kKwBarCount + 16;
+  a.stages = (kKwSmem - rest - 2 * a.n_pad * 256) / kAtTileBytes;
   if (a.stages > kKwMaxStages) a.stages = kKwMaxStages;
-  const int smem = rest + a.q_bufs * a.n_pad * 256 + a.stages * kAtTileBytes;
+  const int smem = rest + 2 * a.n_pad * 256 + a.stages * kAtTileBytes;
   CUtensorMap map_q, map_k;
   if (!encode_queries(w.q, static_cast<int64_t>(w.bs) * w.block, w.hq, group, a.tokens, &map_q) || !encode_cache(w.k_cache, w.num_pages, w.hkv, &map_k))
     return MDB_ERR_CUDA;
