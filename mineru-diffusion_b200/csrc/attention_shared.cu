@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge(const ShArgs a) {
   float m = -INFINITY, l = 0.f;
   float4 acc[4] = {};
   auto join = [&](const float2 p, const float4 (&v)[4]) {
-    if (p.x == -INFINITY) return;                          // (scores that are all -inf)
+    if (p.x == -INFINITY && p.y == p.y) return;            // (scores that are all -inf; a NaN goes on)
     const float m_new = fmaxf(m, p.x), f = ex2_approx(m - m_new), w = ex2_approx(p.x - m_new);
     m = m_new;
     l = l * f + p.y * w;
@@ -741,7 +741,7 @@ int mdb_attn_block_shared(const mdb_attn_shared_args* args, mdb_stream_t stream)
   ShArgs a = {};
   a.out = static_cast<bf16*>(c.out);
   a.lse = c.lse;
-  a.prefix_len = c.prefix_pages > 0 ? c.prefix_len : nullptr;
+  a.prefix_len = c.prefix_len;
   a.prefix_table = c.prefix_table;
   a.ctx_lens = c.ctx_lens;
   a.block_table = c.block_table;

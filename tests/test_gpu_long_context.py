@@ -388,6 +388,44 @@ def test_shared_prefix_lengths_beyond_the_table(mdb):
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+def test_shared_prefix_queries_that_are_not_numbers(mdb):
+    """A NaN in a query is its own row's, and a key of infinities all rows'."""
+    b = Batch([300, 70], 200, 8, 4, 2, seed=14)
+    want, want_lse = b.call(mdb)
+    b.q[0, 3, 2, 5] = NAN
+    out, lse = b.call(mdb)
+    hit = torch.zeros(2, 8, 4, dtype=torch.bool, device=DEV)
+    hit[0, 3, 2] = True
+    assert bool(out[hit].isnan().all()) and bool(lse[hit].isnan().all())
+    assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
+
+
+def test_caches_beyond_32_bits(mdb):
+    """Pages whose offsets pass 2^32 elements."""
+    hkv, pages = 8, 17000
+    kc, vc = (torch.empty(pages, PAGE, hkv, D, dtype=BF, device=DEV) for _ in range(2))
+    assert kc[-1, 0].data_ptr() - kc.data_ptr() > 2 ** 33
+    b = Batch([300, 70], 200, 8, 16, hkv, seed=15)
+    move = torch.randperm(40, generator=gen(1), device=DEV)[: b.pages] + pages - 40
+    kc[move], vc[move] = b.kc, b.vc
+    want, want_lse = b.call(mdb)
+    weights = mdb.ops.key_weights(b.q, b.kc, want_lse, b.seqlens, b.table)
+    high = lambda t: torch.where(t >= 0, move[t.clamp(min=0).long()].to(I32), t)   # noqa: E731
+    out, lse = mdb.ops.block_attn_shared_prefix(b.q, kc, vc, b.prefix_len, high(b.prefix_table), b.seqlens, high(b.table), want_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert torch.equal(mdb.ops.key_weights(b.q, kc, lse, b.seqlens, high(b.table)), weights)
+    kept, lens, _ = mdb.ops.evict_kvcache(kc, vc, weights, b.seqlens, high(b.table), 100, 10)
+    kept_low, _, _ = mdb.ops.evict_kvcache(b.kc, b.vc, weights, b.seqlens, b.table, 100, 10)
+    assert torch.equal(kept, kept_low)
+    at = b.slots(b.table[0], 100)
+    assert torch.equal(kc.view(-1, hkv, D)[b.slots(high(b.table)[0], 100)], b.kc.view(-1, hkv, D)[at])
+    q, k = (torch.randn(2, h, D, generator=gen(2), device=DEV).to(BF) for h in (2, hkv))
+    inv_freq, _ = mdb.ops.rope_frequencies(D)
+    slots = i32([pages * PAGE - 1, pages * PAGE - 300])
+    mdb.ops.rotary_embed(q, k, torch.arange(2, device=DEV), inv_freq, v=k, k_cache=kc, v_cache=vc, slot_mapping=slots)
+    assert torch.equal(vc.view(-1, hkv, D)[slots.long()], k)
+
+
 def test_shared_prefix_refusals(mdb):
     b = Batch([30, 70], 50, 8, 4, 2)
     f = mdb.ops.block_attn_shared_prefix
@@ -588,6 +626,50 @@ def test_evict_weights_of_all_sorts(mdb):
         assert kept[0, 0].tolist() == want
         assert lens_out.tolist() == [budget, min(12, budget)]
         assert kept[1, 0].tolist() == list(range(min(12, budget))) + [-1] * max(0, budget - 12)
+
+
+def test_evict_to_the_same_table_is_in_place(mdb):
+    p = Pool([700], 2, 64, BF, seed=35)
+    before, w = (p.kc.clone(), p.vc.clone()), p.w.clone()
+    kept, lens_out, w_out = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=p.table)
+    p.check(before, kept, lens_out, w_out, p.table, 400, 30, w)
+
+
+@pytest.mark.parametrize("n", [900, 34000])
+def test_evict_equal_weights(mdb, n):
+    """All alike: the first ones stay, and the recent."""
+    p = Pool([n], 1, 16, BF, seed=36)
+    p.w.fill_(0.25)
+    kept, _, _ = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, n // 2, 100)
+    assert kept[0, 0].tolist() == list(range(n // 2 - 100)) + list(range(n - 100, n))
+
+
+def test_evict_in_a_graph_again_and_again(mdb):
+    """Lengths, weights and rows in place, replayed as a request grows."""
+    p = Pool([600, 600], 2, 64, BF, seed=37)               # pages for the longest it grows to
+    kept, w_out = torch.empty(2, 2, 256, dtype=I32, device=DEV), p.w
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    saved = p.kc.clone(), p.vc.clone(), p.w.clone(), p.seqlens.clone()
+
+    def call():
+        mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 256, 32, weights_out=w_out, seqlens_out=p.seqlens, kept=kept)
+
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for t, v in zip((p.kc, p.vc, p.w, p.seqlens), saved):
+        t.copy_(v)
+    for grown in ([600, 350], [400, 300], [256, 600]):
+        p.seqlens.copy_(i32(grown))
+        p.lens = grown
+        before, w = (p.kc.clone(), p.vc.clone()), p.w.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        p.check(before, kept, p.seqlens, w_out, p.table, 256, 32, w)
 
 
 def test_evict_pages_outside_the_pool(mdb):
