@@ -630,6 +630,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
   }
 }
 
+constexpr int kShJoin = 4;
 // Joins the parts of 32 rows of a key head: prefix, CTAs that went on with it, own keys, CTAs that went on with them, in this order.  A
 // lane per row, 16 channels per warp.
 __global__ void __launch_bounds__(256) attn_shared_merge(const ShArgs a) {
@@ -673,12 +674,22 @@ __global__ void __launch_bounds__(256) attn_shared_merge(const ShArgs a) {
   for (int own = 0; own < 2; ++own) {
     if (len[own] == 0) continue;
     join(first_ml[own], first[own]);
-    for (int c = 1; c <= more[own].y; ++c) {
-      const int64_t cta = more[own].x + c;
-      float4 v[4];
+    for (int c0 = 1; c0 <= more[own].y; c0 += kShJoin) {   // several in flight
+      float4 v[kShJoin][4];
+      float2 ml[kShJoin];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = a.cont_o[(cta * 32 + quad + i) * 256 + place[own]];
-      join(a.cont_ml[cta * 256 + place[own]], v);
+      for (int j = 0; j < kShJoin; ++j) {
+        if (c0 + j > more[own].y) break;
+        const int64_t cta = more[own].x + c0 + j;
+        ml[j] = a.cont_ml[cta * 256 + place[own]];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = a.cont_o[(cta * 32 + quad + i) * 256 + place[own]];
+      }
+#pragma unroll
+      for (int j = 0; j < kShJoin; ++j) {
+        if (c0 + j > more[own].y) break;
+        join(ml[j], v[j]);
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;             // (a NaN stays one)
@@ -760,9 +771,11 @@ int mdb_attn_block_shared(const mdb_attn_shared_args* args, mdb_stream_t stream)
   a.cont_ml = a.main_ml + 2 * rows;
   a.info = reinterpret_cast<int2*>(a.cont_ml + static_cast<int64_t>(sms) * 256);
   CUtensorMap map_qp, map_qo, map_k, map_v;
-  if (!encode_queries(c.q, a.tokens, a.hq, a.group, a.box_p, &map_qp) || !encode_queries(c.q, a.tokens, a.hq, a.group, a.box_o, &map_qo) ||
+  if (!encode_queries(c.q, a.tokens, a.hq, a.group, a.box_p, &map_qp) ||
+      (a.box_o != a.box_p && !encode_queries(c.q, a.tokens, a.hq, a.group, a.box_o, &map_qo)) ||
       !encode_cache(c.k_cache, a.num_pages, a.hkv, &map_k) || !encode_cache(c.v_cache, a.num_pages, a.hkv, &map_v))
     return MDB_ERR_CUDA;
+  if (a.box_o == a.box_p) map_qo = map_qp;
   static PerDeviceOnce attr_once;
   const int dev = attr_once.slot();
   if (dev < 0) return MDB_ERR_CUDA;

@@ -6,6 +6,7 @@ and none has a fallback.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -1055,6 +1056,7 @@ def _paged_args(q, k_cache, cache_seqlens, block_table) -> tuple:
     return bs, block, hq, hkv, pages, d, stride, table_pages
 
 
+@functools.lru_cache(maxsize=256)
 def shared_prefix_workspace_bytes(bs: int, block: int, hq: int, hkv: int) -> int:
     """Scratch bytes of ``block_attn_shared_prefix``."""
     return int(_lib.lib().mdb_attn_shared_workspace_bytes(bs, block, hq, hkv))
@@ -1094,7 +1096,7 @@ def block_attn_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         lse = q.new_empty((bs, block, hq), dtype=torch.float32)
     lib = _lib.lib()
     if workspace is None:
-        room = lib.mdb_attn_shared_workspace_bytes(bs, block, hq, hkv)
+        room = shared_prefix_workspace_bytes(bs, block, hq, hkv)
         workspace = q.new_empty(room, dtype=torch.uint8)
     else:
         room = workspace.numel() * workspace.element_size()
