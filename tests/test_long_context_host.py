@@ -106,7 +106,7 @@ def test_c_entries_refuse_before_any_launch(built):
     assert rotary(n=0) == 0 and lib.mdb_rotary_embed(None, None) == -1
     for o, code in (({"dtype": 2}, -1), ({"rot_dims": 66}, -1), ({"rot_dims": 3}, -1), ({"k": None}, -1), ({"k_out": None}, -1), ({"v": at}, -1), ({"inv_freq": None}, -1),
                     ({"slots": at}, -1), ({"slots": at, "k_cache": at}, -1), ({"slots": at, "k_cache": at, "num_slots": 5, "v": at}, -1), ({"dim": 2048}, -3),
-                    ({"heads": 5000}, -3)):
+                    ({"heads": 70000}, -3)):
         assert rotary(**o) == code, o
 
 
