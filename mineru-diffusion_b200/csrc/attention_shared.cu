@@ -24,7 +24,8 @@
 
 namespace mdb {
 
-// Times: a key tile of one query tile, of two, start and end of a unit; the least share of a CTA.
+// Times: a key tile of one query tile, of two, start and end of a unit; the least share of a CTA.  (5 : 8 : 6 for 6 : 8 : 10, 32 blocks
+// behind 8192 keys: 92 for 95 us; 64 tokens behind 16384: 100 for 103.)
 constexpr uint32_t kShOneStep = 5, kShTwoStep = 8, kShUnit = 6, kShMinShare = 16;
 
 struct ShPlan {
@@ -716,8 +717,9 @@ static void sh_units(ShArgs& a, int sms) {
   const int tiles_p = (a.tokens + a.box_p - 1) / a.box_p;
   a.box_o = a.block < most ? a.block : most;
   const int tiles_o = (a.block + a.box_o - 1) / a.box_o;
-  // two tiles to a unit share the reading of the keys and the time of the products; one by one they spread over more SMs
-  a.per_p = tiles_p > 1 && static_cast<int64_t>(a.hkv) * tiles_p * a.prefix_pages * (kPage / kAtKeys) >= 4ll * sms ? 2 : 1;
+  // two tiles to a unit share the reading of the keys and the time of the products; one by one they spread over more SMs.  In key tiles
+  // per SM (4.3: 23.5 us one by one, 26.5 in twos; 7: 24.6, 27.0; 14: 36.4, 36.1)
+  a.per_p = tiles_p > 1 && static_cast<int64_t>(a.hkv) * tiles_p * a.prefix_pages * (kPage / kAtKeys) >= 14ll * sms ? 2 : 1;
   a.per_o = tiles_o > 1 ? 2 : 1;
   a.units_p = (tiles_p + a.per_p - 1) / a.per_p;
   a.units_o = (tiles_o + a.per_o - 1) / a.per_o;
