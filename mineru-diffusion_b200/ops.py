@@ -994,10 +994,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if inv_freq.dtype is not torch.float64 or 2 * pairs > d or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 vector of at most half as many entries as a head has channels")
     if q_out is None:
-        q_out = q.new_empty((n, hq, d))
-        qo_row, qo_head = hq * d, d
-    else:
-        _, qo_row, qo_head = _heads_strides(q_out, n, d, dtype, "q_out", hq)
+        q_out = torch.empty_like(q)              # (of a view of a wider tensor: contiguous)
+    _, qo_row, qo_head = _heads_strides(q_out, n, d, dtype, "q_out", hq)
     hkv, k_row, k_head = (0, 0, 0) if k is None else _heads_strides(k, n, d, dtype, "k")
     v_row = v_head = ko_row = ko_head = slots = 0
     if slot_mapping is not None:
@@ -1168,16 +1166,16 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.T
     for t in (cache_seqlens, seqlens_out):
         if t is not None and (t.dtype is not torch.int32 or t.numel() < bs or not t.is_contiguous()):
             raise ValueError("cache_seqlens and seqlens_out must hold one contiguous int32 per request")
-    if weights_out is None:
-        weights_out = weights.new_empty((bs, hkv, budget))
-    elif weights_out.dim() != 3 or weights_out.dtype is not torch.float32 or weights_out.shape[:2] != (bs, hkv) or weights_out.shape[2] < budget or weights_out.stride(2) != 1:
-        raise ValueError("weights_out must be fp32 [bs, Hkv, at least budget] with a dense last dimension")
-    if seqlens_out is None:
-        seqlens_out = cache_seqlens.new_empty(bs)
     if kept is None:
         kept = cache_seqlens.new_empty((bs, hkv, budget))
     elif kept.shape != (bs, hkv, budget) or kept.dtype is not torch.int32 or not kept.is_contiguous():
         raise ValueError("kept must be contiguous int32 [bs, Hkv, budget]")
+    if weights_out is None:
+        weights_out = torch.empty_like(kept, dtype=torch.float32)
+    elif weights_out.dim() != 3 or weights_out.dtype is not torch.float32 or weights_out.shape[:2] != (bs, hkv) or weights_out.shape[2] < budget or weights_out.stride(2) != 1:
+        raise ValueError("weights_out must be fp32 [bs, Hkv, at least budget] with a dense last dimension")
+    if seqlens_out is None:
+        seqlens_out = torch.empty_like(cache_seqlens) if cache_seqlens.shape == (bs,) else cache_seqlens.new_empty(bs)
     o_row, o_head, _ = weights_out.stride()
     args = _pack_evict(
         bs, hkv, d * k_cache.element_size(), budget, recent, pages, stride, table_pages, out_stride, out_pages, k_cache.data_ptr(), v_cache.data_ptr(),

@@ -178,6 +178,12 @@ def test_rotary_refusals(mdb):
                 lambda: r(q, k, p, f, k_cache=cache.to(BF), slot_mapping=slots), lambda: r(q.transpose(1, 2), None, p, f)):
         with pytest.raises((ValueError, TypeError)):
             bad()
+    with pytest.raises(mdb._lib.MdbError):
+        r(q, None, p, f, q_out=q[:, :1].clone().expand(-1, 2, -1))
+    # layouts other than rows of heads: the output takes the input's
+    turned = torch.randn(2, 4, 64, device=DEV).transpose(0, 1)
+    check_turn(r(turned, None, p, f)[0], turned, p, f, False)
+    check_turn(r(k.expand(-1, 3, -1), None, p, f)[0], k.expand(-1, 3, -1), p, f, False)
     with pytest.raises(TypeError):
         r(q.half(), None, p, f)
     with pytest.raises(RuntimeError):

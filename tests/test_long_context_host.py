@@ -96,7 +96,7 @@ def test_c_entries_refuse_before_any_launch(built):
         assert evict(**o) == code, o
 
     def rotary(**o):
-        a = built._lib.RotaryEmbedArgs(dtype=0, n=2, heads=2, kv_heads=1, dim=64, rot_dims=64)
+        a = built._lib.RotaryEmbedArgs(dtype=0, n=2, heads=2, kv_heads=1, dim=64, rot_dims=64, q_out_row=128, q_out_head=64, k_out_row=64, k_out_head=64)
         for n in ("q", "k", "positions", "inv_freq", "q_out", "k_out"):
             setattr(a, n, at)
         for n, v in o.items():
@@ -106,7 +106,7 @@ def test_c_entries_refuse_before_any_launch(built):
     assert rotary(n=0) == 0 and lib.mdb_rotary_embed(None, None) == -1
     for o, code in (({"dtype": 2}, -1), ({"rot_dims": 66}, -1), ({"rot_dims": 3}, -1), ({"k": None}, -1), ({"k_out": None}, -1), ({"v": at}, -1), ({"inv_freq": None}, -1),
                     ({"slots": at}, -1), ({"slots": at, "k_cache": at}, -1), ({"slots": at, "k_cache": at, "num_slots": 5, "v": at}, -1), ({"dim": 2048}, -3),
-                    ({"heads": 70000}, -3)):
+                    ({"heads": 70000}, -3), ({"q_out_row": 0}, -1), ({"q_out_head": 0}, -1), ({"k_out_row": 0}, -1)):
         assert rotary(**o) == code, o
 
 
