@@ -54,16 +54,25 @@ __device__ __forceinline__ uint32_t ev_before(uint32_t mine, uint32_t* warp_sums
 // Keys of weights [base, base + kEvPage) of the `front` ones, four neighbours at a time: k[4 q + c] is number base + q kEvStride + 4 tid
 // + c.  0, the lowest, behind the last: such a one counts among the lowest and lies behind all of them, so it never stays.
 __device__ __forceinline__ void ev_load(const float* w, int base, int front, bool wide, uint32_t (&k)[4 * kEvQuads]) {
+  const int i0 = base + 4 * static_cast<int>(threadIdx.x);
+  // all loads first: one trip to memory, not one for every four
+#pragma unroll
+  for (int q = 0; q < kEvQuads; ++q) {
+    const int i = i0 + q * kEvStride;
+    if (wide && i + 3 < front) {
+      const uint4 v = *reinterpret_cast<const uint4*>(w + i);
+      k[4 * q] = v.x; k[4 * q + 1] = v.y; k[4 * q + 2] = v.z; k[4 * q + 3] = v.w;
+    }
+  }
 #pragma unroll
   for (int q = 0; q < kEvQuads; ++q) {
     if (base + q * kEvStride >= front) break;
-    const int i = base + q * kEvStride + 4 * static_cast<int>(threadIdx.x);
-    if (wide && i + 3 < front) {
-      const float4 v = *reinterpret_cast<const float4*>(w + i);
-      k[4 * q] = ev_key(v.x); k[4 * q + 1] = ev_key(v.y); k[4 * q + 2] = ev_key(v.z); k[4 * q + 3] = ev_key(v.w);
-    } else {
+    const int i = i0 + q * kEvStride;
+    const bool there = wide && i + 3 < front;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) k[4 * q + c] = i + c < front ? ev_key(w[i + c]) : 0u;
+    for (int c = 0; c < 4; ++c) {
+      if (!there) k[4 * q + c] = i + c < front ? __float_as_uint(w[i + c]) : 0x7fffffffu;      // (a NaN: 0)
+      k[4 * q + c] = ev_key(__uint_as_float(k[4 * q + c]));
     }
   }
 }
@@ -171,17 +180,20 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_k
         if (base + q * kEvStride >= front) break;
         const uint32_t in_front = page + quad_sums[q * 32 + warp] + before[q];
         page += warp_sums[0][q];
-        uint32_t ties = done_equals + (in_front >> 16);
-        uint32_t at = done + (in_front & 0xffffu) + min(ties, equals);
+        uint32_t ties = done_equals + (in_front >> 16), keep = above >> (4 * q) & 15u;
+        const uint32_t at = done + (in_front & 0xffffu) + min(ties, equals), tied = same >> (4 * q) & 15u;
+        if (tied) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (tied >> c & 1) keep |= static_cast<uint32_t>(ties++ < equals) << c;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const bool tie = same >> (4 * q + c) & 1;
-          if ((above >> (4 * q + c) & 1) || (tie && ties < equals)) {
-            kept[at] = base + q * kEvStride + 4 * tid + c;
-            if (w_out != nullptr) w_out[at] = ev_number(k[4 * q + c]);
-            ++at;
+          const uint32_t to = at + __popc(keep & ((1u << c) - 1u));
+          if (keep >> c & 1) {
+            kept[to] = base + q * kEvStride + 4 * tid + c;
+            if (w_out != nullptr) w_out[to] = ev_number(k[4 * q + c]);
           }
-          ties += tie;
         }
       }
       done += page & 0xffffu;
