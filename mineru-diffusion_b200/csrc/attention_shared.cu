@@ -14,12 +14,19 @@
 // such part at most: its first); info[unit] says how many CTAs follow.
 //
 // Roles: a warp that works out the CTA's parts and hands them on through shared memory, a TMA warp (query tiles, rings of K and V
-// tiles), an MMA warp, two groups of four softmax warps, a row per thread.  Units of two tiles take both groups; units of one take them in turn, each with the query tile, the output columns and the barriers of its
-// group, so that one's start lies under the other's end.
+// tiles), an MMA warp, two groups of four softmax warps, a row per thread.  Units of two tiles take
+// both groups; units of one take them in turn, each with the query tile, the output columns and the barriers of its group, so that
+// one's start lies under the other's end.
 // Tensor memory: S_0 (P_0) | S_1 (P_1) | O_0 | O_1, 128 columns each.  Of two tiles each has its score columns, of one it takes both in
 // turn, the next scores ahead of P V.  P goes back into the columns its scores came from, in two halves, of which the first is
 // multiplied while the second is made.  The products of one thread run in the order of issue, so scores may follow a P V into
 // the same columns without a wait.
+//
+// What bounds it.  Two tiles: the chain scores -> maximum and weights (2050 cycles) -> products and next scores (1450), 3500 cycles a round for
+// 2100 of products, and the power limit: 64 blocks of 32 tokens, 16 query and 8 key heads, behind 16384 keys and 1024 to 2048 own ones 322 us
+// alone (930 TFLOP/s), 387 in a loop at 1.5 GHz.  One tile: memory, 64 x 16384 own keys at 5.9 TB/s.  A small batch: latency, 17 us for four
+// blocks behind 1056 keys, of which the joining kernel 5.  No gain from a polynomial for some of the exponentials, nor from other
+// splits of P.
 #include "mdb_common.cuh"
 
 namespace mdb {

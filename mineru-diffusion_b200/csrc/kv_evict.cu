@@ -12,7 +12,9 @@
 //                         new place is never behind its old one, so a CTA that has a slice of the channels of all rows walks
 //                         them in order, loads of a step in front of its stores.
 //
-// Bound by memory: rows read and written once.
+// Bound by memory: rows read and written once.  16 requests of 16384 to 32768 keys, eight heads, 8192 stay: 166 us = 6.4 TB/s for the
+// rows (places looked up by every piece, heads one behind the other: 297), 23 us for the selection in front of them (31 before its
+// weights stayed in registers).
 #include "mdb_common.cuh"
 
 namespace mdb {

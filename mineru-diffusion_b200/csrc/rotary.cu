@@ -7,8 +7,10 @@
 // off by up to 2^-8 radian.  What is left is a number in [-1, 1] half turns, whose sine and cosine need no reduction.
 //
 // A CTA takes some tokens: sines and cosines of their pairs once, into shared memory, for all heads.  A thread has one piece of 16 bytes
-// (half layout: two) of one head, whose place it works out once, and goes through the tokens with it, loads of kReBatch tokens in
-// front of their stores.  It is bound by memory.
+// (half layout: two) of one head, whose place it works out once, and goes through the tokens with it, loads of kReBatch tokens (half
+// layout: of half as many) in front of their stores.  It is bound by memory: 16384 tokens of 40 heads, a quarter of 128 channels turned,
+// 56.5 us = 5.9 TB/s (indices worked out for every token: 66); less than a round of CTAs by the trip to positions, sines and rows (32
+// tokens: 2.7 us).
 #include "mdb_common.cuh"
 
 namespace mdb {
