@@ -23,6 +23,7 @@ namespace mdb {
 constexpr int kKwGroups = 4, kKwThreads = 128 * kKwGroups + 64;       // groups of four warps; TMA, MMA
 constexpr int kKwMaxRows = 512 / kKwGroups;                // rows of a block: the groups' scores fill tensor memory
 constexpr int kKwSegTiles = 16;                            // tiles walked at a time where there are several blocks of rows
+static_assert(kKwSegTiles % kKwGroups == 0, "a group's tiles of a run");
 constexpr int kKwMaxStages = 6;
 constexpr int kKwSmem = 226 * 1024;
 
@@ -278,8 +279,10 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           const float2 p = unpack2(add2(add2(part[0], part[1]), add2(part[2], part[3])));
           acc += p.x + p.y;
           if (a.row_blocks > 1) {
-            if (rb > 0) acc += sums[j * kAtKeys + tid];
-            if (!last_block) sums[j * kAtKeys + tid] = acc;
+            // (a place of the group's own: another group may have gone on to the next run's first block of rows)
+            float& sum = sums[(wg * (kKwSegTiles / kKwGroups) + j / kKwGroups) * kAtKeys + tid];
+            if (rb > 0) acc += sum;
+            if (!last_block) sum = acc;
           }
           if (last_block && key < a.cols) a.out[row + key] = key < s.len ? before + acc : 0.f;
         }

@@ -501,6 +501,16 @@ def test_key_weights(mdb, lens, block, hq, hkv):
     assert torch.equal(past, got)
 
 
+@pytest.mark.parametrize("lens,block,hq,hkv", [([247, 93, 232, 268, 215, 57, 245, 28, 250], 100, 32, 16), ([70] * 60, 200, 2, 2), ([130, 1, 300] * 9, 40, 32, 4)])
+def test_key_weights_of_many_short_requests_in_blocks_of_rows(mdb, lens, block, hq, hkv):
+    """More rows than a block for runs of a tile or two: sums of one run's blocks and of the next one's at the same time."""
+    b = Batch(lens, 600, block, hq, hkv, seed=24, scale=0.2)
+    _, lse = b.call(mdb)
+    got = [mdb.ops.key_weights(b.q, b.kc, lse, b.seqlens, b.table) for _ in range(20)]
+    check_weights(b, got[0], lse)
+    assert all(torch.equal(got[0], g) for g in got[1:])
+
+
 def test_key_weights_of_a_row_sum_to_one(mdb):
     b = Batch([500, 33, 256], 300, 32, 8, 4, seed=21)
     _, lse = b.call(mdb)
