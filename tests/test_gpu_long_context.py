@@ -83,6 +83,38 @@ def test_rotary_embed(mdb, n, hq, hkv, dim, rot, interleaved, dtype):
     assert torch.equal(q, qo) and torch.equal(k, before.split([hq * dim, hkv * dim, hkv * dim], 1)[1].unflatten(1, (-1, dim)))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("n,hq,hkv,dim,rot", [(5003, 32, 8, 128, 128), (16384 + 7, 32, 8, 128, 32), (9001, 16, 4, 64, 64)])
+def test_rotary_of_several_tokens_to_a_cta(mdb, n, hq, hkv, dim, rot, interleaved, dtype):
+    """Prompts of which every CTA has 3 to 16 tokens and the last one fewer: out of place, in place, and into the cache."""
+    g = gen(n)
+    qkv = torch.randn(n, (hq + 2 * hkv) * dim, generator=g, device=DEV).to(dtype)
+    q, k, v = (x.unflatten(1, (-1, dim)) for x in qkv.split([hq * dim, hkv * dim, hkv * dim], 1))
+    inv_freq, factor = mdb.ops.rope_frequencies(rot, 1e6, {"type": "yarn", "factor": 4.0, "original_max_position": 32768})
+    positions = torch.randint(0, 131072, (n,), generator=g, device=DEV)
+    turn = dict(interleaved=interleaved, scale=factor)
+    qo, ko = mdb.ops.rotary_embed(q, k, positions, inv_freq, **turn)
+    check_turn(qo, q, positions, inv_freq, interleaved, factor)
+    check_turn(ko, k, positions, inv_freq, interleaved, factor)
+    pages = -(-n // PAGE) + 1
+    slots = torch.randperm(pages * PAGE, generator=g, device=DEV)[:n].to(I32)
+    slots[::7] = -1
+    slots[-3:] = torch.tensor([-1, int(slots[-2]), -1], dtype=I32, device=DEV)
+    kc, vc = (torch.full((pages, PAGE, hkv, dim), NAN, dtype=dtype, device=DEV) for _ in range(2))
+    stored_q, _ = mdb.ops.rotary_embed(q, k, positions, inv_freq, v=v, k_cache=kc, v_cache=vc, slot_mapping=slots, **turn)
+    there = slots >= 0
+    at = slots[there].long()
+    assert torch.equal(stored_q, qo)
+    assert torch.equal(kc.flatten(0, 1)[at], ko[there]) and torch.equal(vc.flatten(0, 1)[at], v[there])
+    rest = torch.ones(pages * PAGE, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert bool(kc.flatten(0, 1)[rest].isnan().all()) and bool(vc.flatten(0, 1)[rest].isnan().all())
+    before = v.clone()
+    mdb.ops.rotary_embed(q, k, positions, inv_freq, q_out=q, k_out=k, **turn)
+    assert torch.equal(q, qo) and torch.equal(k, ko) and torch.equal(v, before)
+
+
 @pytest.mark.parametrize("where", [0, -5, 2 ** 31, 2 ** 40])
 def test_rotary_positions_out_of_the_ordinary(mdb, where):
     x = torch.randn(3, 2, 128, generator=gen(1), device=DEV)
@@ -289,6 +321,29 @@ def test_shared_prefix_of_many_requests(mdb):
     b.check(out, lse)
     again, lse2 = b.call(mdb)
     assert torch.equal(out, again) and torch.equal(lse, lse2)      # one order of sums
+
+
+@pytest.mark.parametrize("lens,prefix,block,hq,hkv", [
+    ([(37 * i) % 300 for i in range(32)], 4100, 32, 16, 8),
+    ([0] * 33, 2200, 32, 16, 8),                                  # 17 tiles: the last one alone in its unit
+    ([(i % 4) * 45 for i in range(63)], 13400, 7, 6, 2),          # tiles that end inside a request, 126 rows each; eleven of them
+    ([5, 0, 131] * 7, 11000, 33, 12, 3),                          # a unit of fewer rows than its tiles have
+])
+def test_shared_prefix_in_units_of_two_tiles(mdb, lens, prefix, block, hq, hkv):
+    """The form of long prefixes behind many rows.  The units that left their mark in the workspace show that it was taken."""
+    b = Batch(lens, prefix, block, hq, hkv, seed=prefix)
+    need = mdb.ops.shared_prefix_workspace_bytes(b.bs, block, hq, hkv)
+    room = torch.full((need,), 0xFF, dtype=torch.uint8, device=DEV)
+    out, lse = b.call(mdb, workspace=room)
+    b.check(out, lse)
+    tokens, most = b.bs * block, 128 // (hq // hkv)
+    tiles = lambda n: -(-n // min(n, most))                        # noqa: E731
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    marks = room[(2 * tokens * hq + 256 * sms) * (D + 2) * 4:].view(I32).view(-1, 2)
+    own = sum(n > 0 for n in lens) * -(-tiles(block) // 2)
+    assert tiles(tokens) > 1 and int((marks[:, 0] >= 0).sum()) == hkv * (own + -(-tiles(tokens) // 2))
+    again, lse2 = b.call(mdb)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
 def test_shared_prefix_scores_of_all_sizes(mdb):
@@ -658,6 +713,36 @@ def test_evict_equal_weights(mdb, n):
     p.w.fill_(0.25)
     kept, _, _ = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, n // 2, 100)
     assert kept[0, 0].tolist() == list(range(n // 2 - 100)) + list(range(n - 100, n))
+
+
+@pytest.mark.parametrize("in_place", [False, True], ids=["pages", "in_place"])
+@pytest.mark.parametrize("n,budget,recent", [(34000, 33000, 700), (34000, 9000, 100), (70000, 50000, 1000), (70000, 66000, 0)])
+def test_evict_by_weights_of_several_passes(mdb, n, budget, recent, in_place):
+    """More weights than a CTA holds at once: few different ones, so that the last that stays has equals on both sides of the
+    32768th, NaN among them, and some stay in every stretch of 32768."""
+    p = Pool([n, 33000], 1, 16, BF, seed=n + budget, extra_lens=[budget, min(33000, budget)])
+    p.w = (p.w.log() * 4).round() / 4
+    p.w[torch.rand(p.w.shape, generator=gen(38), device=DEV) < 0.01] = NAN
+    before, w = (p.kc.clone(), p.vc.clone()), p.w.clone()
+    more = {"weights_out": p.w, "seqlens_out": p.seqlens} if in_place else {"out_table": p.more}
+    kept, lens_out, w_out = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, budget, recent, **more)
+    sure = False
+    for b, length in enumerate((n, 33000)):
+        m, front, values = min(length, budget), length - recent, w[b, 0].tolist()
+        stay = list(range(m))
+        if length > budget:
+            order = sorted(range(front), key=lambda i: (values[i] != values[i], -values[i] if values[i] == values[i] else 0.0, i))
+            last = order[budget - recent - 1]
+            stay = sorted(order[: budget - recent]) + list(range(front, length))
+            equals = [i for i in range(front) if values[i] == values[last]]
+            sure |= equals[0] < 32768 <= equals[-1] and len({i // 32768 for i in stay}) == -(-length // 32768)
+        assert kept[b, 0].tolist() == stay + [-1] * (budget - m) and int(lens_out[b]) == m
+        at = torch.tensor(stay, device=DEV)
+        assert torch.equal(w_out[b, 0, :m].nan_to_num(nan=77.0), w[b, 0, at].nan_to_num(nan=77.0)) and bool((w_out[b, 0, m:budget] == 0).all())
+        src, dst = Batch.slots(p.table[b].clamp(min=0), length)[at], Batch.slots((p.table if in_place else p.more)[b].clamp(min=0), m)
+        for c, c0 in zip((p.kc, p.vc), before):
+            assert torch.equal(c.view(-1, 16)[dst], c0.view(-1, 16)[src])
+    assert sure
 
 
 def test_evict_in_a_graph_again_and_again(mdb):
