@@ -69,6 +69,7 @@ struct ShArgs {
   float4* cont_o;                // [CTA][32][256]
   float2* cont_ml;               // [CTA][256]
   int2* info;                    // [hkv * units_p + bs * hkv * units_o]: CTA of the first part, how many follow
+  int ctas;                      // of the launch that leaves the sums: places in cont_o and cont_ml
 };
 
 // of a group x: Q, O and P V barriers; S and P barriers by group and score columns
@@ -204,6 +205,16 @@ struct ShWalk {
     return false;
   }
 };
+
+// Whether an entry of info names CTAs of the launch.  One that no CTA has written (a wait ran out) holds what the workspace held.
+__host__ __device__ constexpr bool sh_info_there(int first, int followers, int ctas) {
+  return first >= 0 && followers >= 0 && followers < ctas && first < ctas - followers;
+}
+static_assert(sh_info_there(0, 0, 1) && sh_info_there(0, 147, 148) && sh_info_there(147, 0, 148) && sh_info_there(100, 47, 148), "all CTAs of a launch");
+static_assert(!sh_info_there(0, 1, 1) && !sh_info_there(148, 0, 148) && !sh_info_there(100, 48, 148) && !sh_info_there(1, 147, 148), "behind the last CTA");
+static_assert(!sh_info_there(-1, -1, 148) && !sh_info_there(-1, 1, 148) && !sh_info_there(5, -1, 148) && !sh_info_there(0x5a5a5a5a, 0x5a5a5a5a, 148) &&
+                  !sh_info_there(0x7fffffff, 0x7fffffff, 148) && !sh_info_there(0x7fffffff, 1, 148) && !sh_info_there(0, -0x7fffffff - 1, 148),
+              "whatever lay there");
 
 // The same number to one, eight or 32 columns of every lane.
 __device__ __forceinline__ void tmem_fill1(uint32_t taddr, float v) {
@@ -681,6 +692,14 @@ __global__ void __launch_bounds__(256) attn_shared_merge(const ShArgs a) {
 #pragma unroll
   for (int own = 0; own < 2; ++own) {
     if (len[own] == 0) continue;
+    if (!sh_info_there(more[own].x, more[own].y, a.ctas)) {
+      // the unit has no parts: its row is not a number
+      l = __int_as_float(0x7fffffff);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = make_float4(l, l, l, l);
+      if (quad == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
+      break;
+    }
     join(first_ml[own], first[own]);
     for (int c0 = 1; c0 <= more[own].y; c0 += kShJoin) {   // several in flight
       float4 v[kShJoin][4];
@@ -769,6 +788,7 @@ int mdb_attn_block_shared(const mdb_attn_shared_args* args, mdb_stream_t stream)
   a.bs = c.bs; a.block = c.block; a.hq = c.hq; a.hkv = c.hkv;
   a.scale_log2 = c.softmax_scale * 1.4426950408889634f;
   const int sms = at_sm_count();
+  a.ctas = sms;
   sh_units(a, sms);
   // the list's length is kept in 32 bits (2^32 is minutes of work)
   const int64_t steps = kPage / kAtKeys, most = (a.prefix_pages * steps * kShTwoStep + kShUnit) * a.units_p + (a.table_pages * steps * kShTwoStep + kShUnit) * a.units_o * a.bs;
