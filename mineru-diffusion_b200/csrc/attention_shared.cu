@@ -76,7 +76,7 @@ struct ShArgs {
 enum {
   kShBarQFull = 0, kShBarQEmpty = 2, kShBarKFull = 4, kShBarKEmpty = 7, kShBarVFull = 10, kShBarVEmpty = 12, kShBarSFull = 14 /* 2 x + buf */,
   kShBarPDone = 18, kShBarOFull = 20, kShBarOEmpty = 22, kShBarPFull = 24 /* 2 (2 x + buf) + half */, kShBarPartFull = 32,
-  kShBarPartEmpty = 36, kShBarCount = 40
+  kShBarPartEmpty = 36, kShBarEnd = 40 /* of all products */, kShBarCount = 41
 };
 
 __device__ __forceinline__ int sh_prefix(const ShArgs& a) {
@@ -251,7 +251,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
   pdl_launch_dependents();
   if (warp == 0) {
     mbar_init(bar(lane), lane >= kShBarOEmpty ? 4 : 1);      // (the softmax warps' are the last ones of these)
-    if (lane < kShBarCount - 32) mbar_init(bar(32 + lane), 32 + lane >= kShBarPartEmpty ? 10 : 1);
+    if (lane < kShBarCount - 32) mbar_init(bar(32 + lane), 32 + lane >= kShBarPartEmpty && 32 + lane < kShBarEnd ? 10 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -332,13 +332,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
           }
           if (!ok) break;
         }
-        if (!ok) {
-          report_status(MDB_STATUS_WAIT_TIMEOUT);
-          // let the copies already issued land before the CTA gives its shared memory back
-          for (int s = 0; s < P::kKStages; ++s) if (pend_k >> s & 1) mbar_wait(bar(kShBarKFull + s), par_k >> s & 1);
-          for (int s = 0; s < P::kVStages; ++s) if (pend_v >> s & 1) mbar_wait(bar(kShBarVFull + s), par_v >> s & 1);
-          for (int s = 0; s < 2; ++s) if (pend_q >> s & 1) mbar_wait(bar(kShBarQFull + s), par_q >> s & 1);
-        }
+        if (!ok) report_status(MDB_STATUS_WAIT_TIMEOUT);
+        // let the copies issued land before the CTA gives its shared memory back: another warp may have given up waiting for them
+        for (int s = 0; s < P::kKStages; ++s) if (pend_k >> s & 1) mbar_wait(bar(kShBarKFull + s), par_k >> s & 1);
+        for (int s = 0; s < P::kVStages; ++s) if (pend_v >> s & 1) mbar_wait(bar(kShBarVFull + s), par_v >> s & 1);
+        for (int s = 0; s < 2; ++s) if (pend_q >> s & 1) mbar_wait(bar(kShBarQFull + s), par_q >> s & 1);
       }
     } else if (warp == kMmaWarp) {
       // ----------------------------------------------------------------- MMA issue (all lanes, one elected)
@@ -457,6 +455,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_qp, const __grid_cons
         }
       }
       if (!ok && lane == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
+      // the products issued end before the CTA gives its memories back: this warp or another one may have given up waiting for them
+      umma_commit_w(bar(kShBarEnd));
+      mbar_wait_w(bar(kShBarEnd), 0);
     } else if (warp == kPartsWarp) {
       // ----------------------------------------------------------------- the CTA's parts
       ShWalk walk;

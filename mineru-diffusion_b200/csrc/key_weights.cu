@@ -113,7 +113,7 @@ struct KwWalk {
 // barrier slots
 enum {
   kKwBarQFull = 0, kKwBarQEmpty = 2, kKwBarSFull = 4, kKwBarSEmpty = kKwBarSFull + kKwGroups, kKwBarKFull = kKwBarSEmpty + kKwGroups,
-  kKwBarKEmpty = kKwBarKFull + kKwMaxStages, kKwBarCount = kKwBarKEmpty + kKwMaxStages
+  kKwBarKEmpty = kKwBarKFull + kKwMaxStages, kKwBarEnd = kKwBarKEmpty + kKwMaxStages /* of all products */, kKwBarCount
 };
 
 __global__ void __launch_bounds__(kKwThreads, 1)
@@ -183,11 +183,10 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           }
         }
       }
-      if (!ok) {
-        report_status(MDB_STATUS_WAIT_TIMEOUT);
-        for (int i = 0; i < a.stages; ++i) if (pend_k >> i & 1) mbar_wait(bar(kKwBarKFull + i), par_k >> i & 1);
-        for (int i = 0; i < 2; ++i) if (pend_q >> i & 1) mbar_wait(bar(kKwBarQFull + i), par_q >> i & 1);
-      }
+      if (!ok) report_status(MDB_STATUS_WAIT_TIMEOUT);
+      // let the copies issued land before the CTA gives its shared memory back: another warp may have given up waiting for them
+      for (int i = 0; i < a.stages; ++i) if (pend_k >> i & 1) mbar_wait(bar(kKwBarKFull + i), par_k >> i & 1);
+      for (int i = 0; i < 2; ++i) if (pend_q >> i & 1) mbar_wait(bar(kKwBarQFull + i), par_q >> i & 1);
     }
   } else if (warp == kMmaWarp) {
     const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a.n_pad >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
@@ -219,6 +218,9 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       seg_base += s.tiles;
     }
     if (!ok && lane == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
+    // the products issued end before the CTA gives its memories back: this warp or another one may have given up waiting for them
+    umma_commit_w(bar(kKwBarEnd));
+    mbar_wait_w(bar(kKwBarEnd), 0);
   } else {
     const int wg = warp >> 2, tid = threadIdx.x & 127;     // (tid: tensor-memory lane, key of a tile)
     const uint32_t lane_field = static_cast<uint32_t>(32 * (warp & 3)) << 16;
