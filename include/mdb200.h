@@ -778,7 +778,8 @@ int mdb_key_weights(const mdb_key_weights_args* args, mdb_stream_t stream);
  * Their rows of row_bytes bytes (a multiple of 16) in K and V, and their weights, move in order to the first places of the
  * request's pages (out_table NULL) or of the pages in out_table, which hold none of those read.  Pages that are written
  * belong to one request.  kept [bs][kv_heads][budget] = old places, -1 behind the last; weights_out (may be NULL, may be
- * weights) gets 0 there; seqlens_out (may be seqlens) = min(seqlens, budget). */
+ * weights) gets 0 there, and behind the budget in all of its columns: of these it has weight_cols where it is weights (strides too) and
+ * budget otherwise, or as many as mdb_kv_evict_wide is told (at least budget).  seqlens_out (may be seqlens) = min(seqlens, budget). */
 typedef struct {
   int32_t bs, kv_heads, row_bytes, budget, recent, num_pages, table_stride, table_pages, out_table_stride, out_table_pages;
   void* k_cache;
@@ -794,6 +795,7 @@ typedef struct {
   int32_t* kept;
 } mdb_kv_evict_args;
 int mdb_kv_evict(const mdb_kv_evict_args* args, mdb_stream_t stream);
+int mdb_kv_evict_wide(const mdb_kv_evict_args* args, int64_t weight_out_cols, mdb_stream_t stream);
 
 #ifdef __cplusplus
 }

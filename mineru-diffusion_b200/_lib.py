@@ -190,6 +190,7 @@ SIGNATURES = {
     "mdb_attn_block_shared": (_i, [_p, _p]),
     "mdb_key_weights": (_i, [_p, _p]),
     "mdb_kv_evict": (_i, [_p, _p]),
+    "mdb_kv_evict_wide": (_i, [_p, _i64, _p]),
     "mdb_pick_token": (_i, [_p, _i64, _i, _i, _p, _u32, _p, _p, _p, _p]),
 }
 

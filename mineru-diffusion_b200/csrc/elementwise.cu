@@ -444,7 +444,7 @@ const char* mdb_strerror(int code) {
   }
 }
 
-int mdb_version(void) { return 104; }
+int mdb_version(void) { return 105; }
 
 int mdb_set_trace(void* buffer, int64_t bytes) {
   TraceBuf t;

@@ -79,7 +79,8 @@ __device__ __forceinline__ void ev_load(const float* w, int base, int front, boo
   }
 }
 
-__global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_kv_evict_args a) {
+// out_cols: of weights_out.
+__global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_kv_evict_args a, const int64_t out_cols) {
   __shared__ uint32_t counts[kEvBins];
   __shared__ uint32_t warp_sums[2][32];
   __shared__ uint32_t quad_sums[kEvQuads * 32];
@@ -214,6 +215,10 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_k
     }
     __syncthreads();
   }
+  // Behind the budget lie no keys: with weights_out the weights, what lay there would be the past of keys that are appended later.  (All of
+  // w has been read.)
+  if (w_out != nullptr)
+    for (int64_t i = a.budget + tid; i < out_cols; i += kEvThreads) w_out[i] = 0.f;
 }
 
 // Byte offset of a place in the pool, or -1.
@@ -291,11 +296,19 @@ using namespace mdb;
 
 extern "C" int mdb_kv_evict(const mdb_kv_evict_args* args, mdb_stream_t stream) {
   MDB_REQUIRE(args != nullptr, MDB_ERR_ARG);
+  const mdb_kv_evict_args& a = *args;
+  const bool same = a.weights_out == a.weights && a.weight_out_row == a.weight_row && a.weight_out_head == a.weight_head && a.weight_cols > a.budget;
+  return mdb_kv_evict_wide(args, same ? a.weight_cols : a.budget, stream);
+}
+
+extern "C" int mdb_kv_evict_wide(const mdb_kv_evict_args* args, int64_t weight_out_cols, mdb_stream_t stream) {
+  MDB_REQUIRE(args != nullptr, MDB_ERR_ARG);
   const mdb_kv_evict_args a = *args;
   MDB_REQUIRE(a.bs >= 0 && a.kv_heads > 0 && a.row_bytes > 0 && a.budget > 0 && a.recent >= 0 && a.recent <= a.budget && a.num_pages > 0 &&
                   a.table_pages > 0 && (a.table_stride >= a.table_pages || a.bs <= 1) && a.weight_cols > 0,
               MDB_ERR_ARG);
   if (a.bs == 0) return MDB_OK;
+  MDB_REQUIRE(a.weights_out == nullptr || weight_out_cols >= a.budget, MDB_ERR_ARG);
   MDB_REQUIRE(a.k_cache && a.v_cache && a.weights && a.seqlens && a.seqlens_out && a.block_table && a.kept, MDB_ERR_ARG);
   MDB_REQUIRE(a.out_table == nullptr || (a.out_table_pages > 0 && (a.out_table_stride >= a.out_table_pages || a.bs <= 1)), MDB_ERR_ARG);
   MDB_REQUIRE(a.row_bytes % 16 == 0 && mdb_aligned16(a.k_cache) && mdb_aligned16(a.v_cache), MDB_ERR_ALIGN);
@@ -303,7 +316,7 @@ extern "C" int mdb_kv_evict(const mdb_kv_evict_args* args, mdb_stream_t stream) 
               MDB_ERR_UNSUPPORTED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int pairs = a.bs * a.kv_heads;
-  int rc = mdb_launch(evict_select_kernel, dim3(pairs), dim3(kEvThreads), 0, st, a);
+  int rc = mdb_launch(evict_select_kernel, dim3(pairs), dim3(kEvThreads), 0, st, a, weight_out_cols);
   if (rc != MDB_OK) return rc;
   // slices of a power of two of pieces that divides the row, as wide as it goes; in place narrower, down to 32 bytes, until the
   // SMs have two CTAs each (one request of 4100 keys, eight heads: 28 us whole rows, 15 us slices; 16 of 8192 alike)

@@ -1140,8 +1140,8 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.T
     lowest index wins a tie).  The rows of K and V that stay are packed in order into the first places of the request's pages, or
     of the pages in ``out_table`` (int32 [bs, pages], none of the pages read: for pages that others still read, as a shared
     prefix's); written pages must belong to one request.  Returns (kept int32 [bs, Hkv, budget] = old places, -1 behind the last;
-    new lengths int32 [bs]; weights of the kept keys [bs, Hkv, >= budget], 0 behind the last).  ``weights_out`` may be ``weights`` and
-    ``seqlens_out`` may be ``cache_seqlens``."""
+    new lengths int32 [bs]; weights of the kept keys [bs, Hkv, >= budget], 0 in all columns behind the last).  ``weights_out`` may be
+    ``weights`` (keys that are appended later then start from 0) and ``seqlens_out`` may be ``cache_seqlens``."""
     _all_here(k_cache, v_cache, weights, cache_seqlens, block_table, out_table, weights_out, seqlens_out, kept)
     if k_cache.dtype not in _DTYPES:
         raise TypeError(f"k_cache must be bfloat16 or float32, got {k_cache.dtype}")
@@ -1181,5 +1181,5 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.T
         bs, hkv, d * k_cache.element_size(), budget, recent, pages, stride, table_pages, out_stride, out_pages, k_cache.data_ptr(), v_cache.data_ptr(),
         weights.data_ptr(), w_row, w_head, cols, weights_out.data_ptr(), o_row, o_head, cache_seqlens.data_ptr(), seqlens_out.data_ptr(),
         block_table.data_ptr(), 0 if out_table is None else out_table.data_ptr(), kept.data_ptr())
-    _lib.check(_lib.lib().mdb_kv_evict(args, _stream()), "mdb_kv_evict")
+    _lib.check(_lib.lib().mdb_kv_evict_wide(args, weights_out.shape[2], _stream()), "mdb_kv_evict_wide")
     return kept, seqlens_out, weights_out

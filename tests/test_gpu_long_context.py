@@ -773,6 +773,38 @@ def test_evict_in_a_graph_again_and_again(mdb):
         p.check(before, kept, p.seqlens, w_out, p.table, 256, 32, w)
 
 
+@pytest.mark.parametrize("lens,budget,recent", [([700, 90, 0], 200, 30), ([40000, 300], 20000, 0)])
+def test_evict_leaves_no_weight_behind_the_last_key(mdb, lens, budget, recent):
+    """Weights in place or in wider columns: keys appended later have no past."""
+    p = Pool(lens, 2, 16, BF, seed=39)
+    want = mdb.ops.evict_kvcache(p.kc.clone(), p.vc.clone(), p.w, p.seqlens, p.table, budget, recent)[2]
+    cols = p.w.shape[2]
+    beside = torch.full((len(lens), 2, cols + 40), 5.0, device=DEV)
+    for room in (p.w.clone(), beside[..., : cols + 7], p.w):
+        _, _, got = mdb.ops.evict_kvcache(p.kc.clone(), p.vc.clone(), p.w, p.seqlens, p.table, budget, recent, weights_out=room)
+        assert got is room
+        assert torch.equal(got[..., :budget], want) and bool((got[..., budget:] == 0).all())
+    assert bool((beside[..., cols + 7:] == 5.0).all())
+
+
+def test_weights_of_keys_that_follow_an_eviction(mdb):
+    """One buffer of weights for a request that shrinks and grows again."""
+    b = Batch([500, 90], 0, 8, 4, 2, seed=40)
+    _, lse = b.call(mdb)
+    weights = mdb.ops.key_weights(b.q, b.kc, lse, b.seqlens, b.table)
+    mdb.ops.evict_kvcache(b.kc, b.vc, weights, b.seqlens, b.table, 100, 20, weights_out=weights, seqlens_out=b.seqlens)
+    b.lens = [300, 290]                                    # the pages hold keys there
+    b.kc.nan_to_num_(0.25, 0.25, 0.25)
+    b.vc.nan_to_num_(0.25, 0.25, 0.25)
+    b.table[1, 1] = b.prefix_table[0]                      # (nobody's: the prefix is empty)
+    b.seqlens.copy_(i32(b.lens))
+    past = weights.clone()
+    past[0, :, 100:] = past[1, :, 90:] = 0
+    _, lse = b.call(mdb)
+    mdb.ops.key_weights(b.q, b.kc, lse, b.seqlens, b.table, previous=weights, decay=0.5, out=weights)
+    check_weights(b, weights, lse, past, 0.5)
+
+
 def test_evict_pages_outside_the_pool(mdb):
     p = Pool([600, 300], 2, 64, BF, seed=32)
     before = p.kc.clone()

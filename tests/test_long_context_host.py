@@ -110,6 +110,21 @@ def test_c_entries_refuse_before_any_launch(built):
         assert rotary(**o) == code, o
 
 
+def test_eviction_with_wide_weights_refused(built):
+    lib, at = built._lib.lib(), 64
+
+    def wide(cols, **o):
+        a = built._lib.KvEvictArgs(bs=1, kv_heads=2, row_bytes=256, budget=10, recent=2, num_pages=4, table_stride=2, table_pages=2, weight_cols=100)
+        for n in ("k_cache", "v_cache", "weights", "weights_out", "seqlens", "seqlens_out", "block_table", "kept"):
+            setattr(a, n, at)
+        for n, v in o.items():
+            setattr(a, n, v)
+        return lib.mdb_kv_evict_wide(ctypes.byref(a), cols, None)
+
+    assert wide(10, bs=0) == 0 and lib.mdb_kv_evict_wide(None, 10, None) == -1
+    assert wide(9) == -1 and wide(0) == -1 and wide(100, row_bytes=24) == -2 and wide(0, weights_out=None, row_bytes=24) == -2
+
+
 def test_workspace_of_the_shared_prefix(built):
     need = built.ops.shared_prefix_workspace_bytes
     assert need(0, 32, 16, 8) == 0 and need(4, 32, 16, 5) == 0
