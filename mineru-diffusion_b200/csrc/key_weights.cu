@@ -239,11 +239,13 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       for (int rb = 0; rb < a.row_blocks && ok; ++rb) {
         const int tok0 = rb * a.tokens, rows = min(a.tokens, a.block - tok0) * a.group;
         __syncwarp();
+        bool none = false;             // a row that saw no key gives none a weight, whatever its query holds
         for (int r = lane; r < rows; r += 32) {
           const float l = a.lse[(static_cast<int64_t>(s.b) * a.block + tok0 + r / a.group) * a.hq + s.h * a.group + r % a.group];
-          neg_lse[r] = l * -1.4426950408889634f;
-          if (l == -INFINITY) neg_lse[r] = -INFINITY;      // a row that saw no key gives none a weight
+          neg_lse[r] = l == -INFINITY ? -INFINITY : l * -1.4426950408889634f;
+          none |= l == -INFINITY;
         }
+        none = __any_sync(0xffffffffu, none);
         __syncwarp();
         for (int j = 0; j < s.tiles; ++j) {
           if (static_cast<int>((seg_base + j) % kKwGroups) != wg) continue;
@@ -260,7 +262,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             float x[32];
             tmem_ld32(tmem_base + wg * kKwMaxRows + lane_field + c, x);      // (columns behind the last row are not looked at)
             tmem_ld_wait();
-            if (c + 32 <= rows) {
+            if (c + 32 <= rows && !none) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float4 n = *reinterpret_cast<const float4*>(neg_lse + c + i);
@@ -272,7 +274,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             } else {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (c + i < rows) acc += ex2_approx(fmaf(x[i], a.scale_log2, neg_lse[c + i]));
+                if (c + i < rows && neg_lse[c + i] != -INFINITY) acc += ex2_approx(fmaf(x[i], a.scale_log2, neg_lse[c + i]));
             }
           }
           tc_fence_before();

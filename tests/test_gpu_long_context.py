@@ -585,6 +585,29 @@ def test_key_weights_of_rows_that_saw_nothing(mdb):
     assert bool((got[1] == 0).all())
 
 
+@pytest.mark.parametrize("block,hq,hkv", [(8, 4, 2), (32, 16, 8), (32, 8, 4), (100, 6, 2)])
+def test_key_weights_of_padded_rows(mdb, block, hq, hkv):
+    """Rows of lse -inf whose queries hold NaN and infinities, as padding does."""
+    b = Batch([300, 64, 700], 50, block, hq, hkv, seed=25)
+    _, lse = b.call(mdb)
+    pad = torch.zeros(3, block, dtype=torch.bool, device=DEV)
+    pad[0, 3] = pad[1, block // 2:] = pad[2, ::3] = True
+    clean = b.q.clone()
+    lse[pad] = -math.inf
+    clean[pad] = 0.0
+    want = mdb.ops.key_weights(clean, b.kc, lse, b.seqlens, b.table)
+    b.q[pad] = NAN
+    b.q[0, 3, 0] = math.inf
+    got = mdb.ops.key_weights(b.q, b.kc, lse, b.seqlens, b.table)
+    assert torch.equal(got, want)
+    b.q = clean
+    check_weights(b, got, lse)
+    # a row whose lse is not a number is not padding
+    lse[1, 0, 0] = NAN
+    got = mdb.ops.key_weights(b.q, b.kc, lse, b.seqlens, b.table)
+    assert bool(got[1, 0, :64].isnan().all()) and torch.equal(got[0], want[0]) and torch.equal(got[1, 1:], want[1, 1:])
+
+
 def test_key_weights_bad_pages_and_lengths(mdb):
     b = Batch([300, 70], 50, 8, 4, 2, seed=23)
     _, lse = b.call(mdb)
