@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const mdb_kv
   const int32_t* kept = a.kept + static_cast<int64_t>(pair) * a.budget;
   const int32_t* from = a.block_table + static_cast<int64_t>(b) * a.table_stride;
   const int32_t* to = IN_PLACE ? from : a.out_table + static_cast<int64_t>(b) * a.out_table_stride;
-  const int to_pages = IN_PLACE ? a.table_pages : a.out_table_pages;
+  const int to_pages = a.out_table == nullptr ? a.table_pages : a.out_table_pages;
   const int64_t token_bytes = static_cast<int64_t>(a.kv_heads) * a.row_bytes;
   const int piece = tid % slice, r0 = tid / slice, rows = kEvMoveThreads / slice;
   cache += static_cast<int64_t>(h) * a.row_bytes + (part * slice + piece) * 16;
@@ -323,7 +323,8 @@ extern "C" int mdb_kv_evict_wide(const mdb_kv_evict_args* args, int64_t weight_o
   const int pieces = a.row_bytes / 16;
   int slice = 1;
   while (slice < 32 && pieces % (2 * slice) == 0) slice *= 2;
-  if (a.out_table == nullptr) {
+  // the same table once more: in place (a table that starts at the same entry with rows further apart is another one)
+  if (a.out_table == nullptr || (a.out_table == a.block_table && (a.out_table_stride == a.table_stride || a.bs <= 1))) {
     while (slice > 2 && static_cast<int64_t>(pairs) * 2 * (pieces / slice) < 2 * 148) slice /= 2;
     return mdb_launch(evict_move_kernel<true>, dim3(2 * pairs * (pieces / slice)), dim3(kEvMoveThreads), 0, st, a, slice);
   }

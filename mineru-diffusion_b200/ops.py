@@ -1158,8 +1158,6 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.T
     if not 0 <= recent <= budget or not 1 <= budget <= 1 << 23:
         raise ValueError("budget must be between 1 and 2^23, recent between 0 and budget")
     stride, table_pages = _table_args(block_table, bs)
-    if out_table is not None and out_table.data_ptr() == block_table.data_ptr():
-        out_table = None
     out_stride, out_pages = (0, 0) if out_table is None else _table_args(out_table, bs)
     if out_table is not None and out_pages * 256 < min(budget, table_pages * 256):
         raise ValueError("out_table must have pages for budget keys")

@@ -729,6 +729,31 @@ def test_evict_to_the_same_table_is_in_place(mdb):
     p.check(before, kept, lens_out, w_out, p.table, 400, 30, w)
 
 
+def test_evict_to_a_table_that_starts_with_the_same_row(mdb):
+    """Two views of one tensor, row strides apart: request 1 goes to pages of its own, not back into its old ones."""
+    p = Pool([0, 700], 2, 64, BF, seed=42, extra_lens=[400])
+    both = torch.cat([p.table, torch.full((1, p.table.shape[1]), -1, dtype=I32, device=DEV)])
+    both[2, : p.more.shape[1]] = p.more[0]
+    p.table, to = both[:2], both[::2]
+    assert p.table.data_ptr() == to.data_ptr()
+    before, w = (p.kc.clone(), p.vc.clone()), p.w.clone()
+    kept, lens_out, w_out = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=to)
+    p.check(before, kept, lens_out, w_out, to, 400, 30, w)
+    with pytest.raises(ValueError):                        # as many pages as the budget needs, of any table
+        mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=p.table[:, :1])
+    with pytest.raises(ValueError):
+        mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=p.table[:1])
+
+
+def test_evict_one_request_to_its_own_row(mdb):
+    """A row stride says nothing of a single row."""
+    p = Pool([700], 2, 64, BF, seed=43)
+    before, w = (p.kc.clone(), p.vc.clone()), p.w.clone()
+    to = p.table.as_strided((1, 2), (17, 1))
+    kept, lens_out, w_out = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=to)
+    p.check(before, kept, lens_out, w_out, p.table, 400, 30, w)
+
+
 @pytest.mark.parametrize("n", [900, 34000])
 def test_evict_equal_weights(mdb, n):
     """All alike: the first ones stay, and the recent."""
