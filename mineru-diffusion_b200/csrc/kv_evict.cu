@@ -79,8 +79,8 @@ __device__ __forceinline__ void ev_load(const float* w, int base, int front, boo
   }
 }
 
-// out_cols: of weights_out.
-__global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_kv_evict_args a, const int64_t out_cols) {
+// out_cols: of weights_out; apart: the rows go to other pages, in any order.
+__global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_kv_evict_args a, const int64_t out_cols, const bool apart) {
   __shared__ uint32_t counts[kEvBins];
   __shared__ uint32_t warp_sums[2][32];
   __shared__ uint32_t quad_sums[kEvQuads * 32];
@@ -204,10 +204,23 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_k
       __syncthreads();
     }
   }
+  float y = tid < recent && w_out != nullptr ? w[front + tid] : 0.f;
+  // does the request write a page that it reads?  (looked up here, under the first of these loads: in front of the selection 1 us longer)
+  bool both = false;
+  if (apart) {
+    const int32_t* from = a.block_table + static_cast<int64_t>(b) * a.table_stride;
+    const int32_t* to = a.out_table + static_cast<int64_t>(b) * a.out_table_stride;
+    const int reads = (n + kPage - 1) / kPage, writes = min((min(n, a.budget) + kPage - 1) / kPage, a.out_table_pages);
+    for (int t = lane; t < writes; t += 32) {
+      const int page = to[t];
+#pragma unroll 4
+      for (int r = warp; r < reads; r += kEvThreads / 32) both |= from[r] == page && page >= 0;
+    }
+  }
   for (int base = 0; base < a.budget - need; base += kEvThreads) {
     const int i = base + tid;
     const bool there = i < recent;
-    const float y = there && w_out != nullptr ? w[front + i] : 0.f;
+    if (base > 0) y = there && w_out != nullptr ? w[front + i] : 0.f;
     __syncthreads();
     if (i < a.budget - need) {
       kept[need + i] = there ? front + i : -1;
@@ -215,10 +228,17 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const mdb_k
     }
     __syncthreads();
   }
+  int64_t rest = a.budget;
+  if (apart && __syncthreads_or(both)) {
+    // it keeps nothing, so that no row moves
+    for (int i = tid; i < a.budget; i += kEvThreads) kept[i] = -1;
+    rest = 0;
+    if (tid == 0) report_status(MDB_STATUS_BAD_PAGE);
+  }
   // Behind the budget lie no keys: with weights_out the weights, what lay there would be the past of keys that are appended later.  (All of
   // w has been read.)
   if (w_out != nullptr)
-    for (int64_t i = a.budget + tid; i < out_cols; i += kEvThreads) w_out[i] = 0.f;
+    for (int64_t i = rest + tid; i < out_cols; i += kEvThreads) w_out[i] = 0.f;
 }
 
 // Byte offset of a place in the pool, or -1.
@@ -253,7 +273,8 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const mdb_kv
   if (blockIdx.y == 0 && part == 0 && !values && h == 0 && tid == 0) {
     // (the lengths are read by the kernel in front alone, so that they may be replaced here)
     const int64_t most = min(static_cast<int64_t>(a.table_pages) * kPage, static_cast<int64_t>(a.weight_cols));
-    a.seqlens_out[b] = max(0, static_cast<int>(min(static_cast<int64_t>(min(a.seqlens[b], a.budget)), most)));
+    const int stay = max(0, static_cast<int>(min(static_cast<int64_t>(min(a.seqlens[b], a.budget)), most)));
+    a.seqlens_out[b] = kept[0] < 0 ? 0 : stay;
   }
   bool bad = false;
   for (int base = IN_PLACE ? 0 : blockIdx.y * kEvMoveRows; base < a.budget; base += kRows) {
@@ -316,15 +337,16 @@ extern "C" int mdb_kv_evict_wide(const mdb_kv_evict_args* args, int64_t weight_o
               MDB_ERR_UNSUPPORTED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int pairs = a.bs * a.kv_heads;
-  int rc = mdb_launch(evict_select_kernel, dim3(pairs), dim3(kEvThreads), 0, st, a, weight_out_cols);
+  // the same table once more: in place (a table that starts at the same entry with rows further apart is another one)
+  const bool apart = a.out_table != nullptr && (a.out_table != a.block_table || (a.out_table_stride != a.table_stride && a.bs > 1));
+  int rc = mdb_launch(evict_select_kernel, dim3(pairs), dim3(kEvThreads), 0, st, a, weight_out_cols, apart);
   if (rc != MDB_OK) return rc;
   // slices of a power of two of pieces that divides the row, as wide as it goes; in place narrower, down to 32 bytes, until the
   // SMs have two CTAs each (one request of 4100 keys, eight heads: 28 us whole rows, 15 us slices; 16 of 8192 alike)
   const int pieces = a.row_bytes / 16;
   int slice = 1;
   while (slice < 32 && pieces % (2 * slice) == 0) slice *= 2;
-  // the same table once more: in place (a table that starts at the same entry with rows further apart is another one)
-  if (a.out_table == nullptr || (a.out_table == a.block_table && (a.out_table_stride == a.table_stride || a.bs <= 1))) {
+  if (!apart) {
     while (slice > 2 && static_cast<int64_t>(pairs) * 2 * (pieces / slice) < 2 * 148) slice /= 2;
     return mdb_launch(evict_move_kernel<true>, dim3(2 * pairs * (pieces / slice)), dim3(kEvMoveThreads), 0, st, a, slice);
   }

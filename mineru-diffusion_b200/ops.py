@@ -1139,9 +1139,10 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.T
     stay, and of those in front the ones with the largest ``weights`` (fp32 [bs, Hkv, columns]; NaN counts as the lowest, the
     lowest index wins a tie).  The rows of K and V that stay are packed in order into the first places of the request's pages, or
     of the pages in ``out_table`` (int32 [bs, pages], none of the pages read: for pages that others still read, as a shared
-    prefix's); written pages must belong to one request.  Returns (kept int32 [bs, Hkv, budget] = old places, -1 behind the last;
-    new lengths int32 [bs]; weights of the kept keys [bs, Hkv, >= budget], 0 in all columns behind the last).  ``weights_out`` may be
-    ``weights`` (keys that are appended later then start from 0) and ``seqlens_out`` may be ``cache_seqlens``."""
+    prefix's; a request that would write a page it reads itself keeps nothing, with the bad-page status).  Written pages must
+    belong to one request.  Returns (kept int32 [bs, Hkv, budget] = old places, -1 behind the last; new lengths int32 [bs]; weights
+    of the kept keys [bs, Hkv, >= budget], 0 in all columns behind the last).  ``weights_out`` may be ``weights`` (keys that are
+    appended later then start from 0) and ``seqlens_out`` may be ``cache_seqlens``."""
     _all_here(k_cache, v_cache, weights, cache_seqlens, block_table, out_table, weights_out, seqlens_out, kept)
     if k_cache.dtype not in _DTYPES:
         raise TypeError(f"k_cache must be bfloat16 or float32, got {k_cache.dtype}")

@@ -745,6 +745,31 @@ def test_evict_to_a_table_that_starts_with_the_same_row(mdb):
         mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=p.table[:1])
 
 
+@pytest.mark.parametrize("how", ["copy", "one page", "later page"])
+def test_evict_to_pages_that_are_read(mdb, how):
+    """A copy of the table, or a page of the request's own: told, and the caches are left as they were.  Other requests go on."""
+    p = Pool([700, 500], 2, 64, BF, seed=44, extra_lens=[400, 400])
+    p.more = p.more[:, :2].contiguous()
+    to = p.more.clone()
+    if how == "copy":
+        to[0] = p.table[0, :2]
+    else:
+        to[0, 1] = p.table[0, 0 if how == "one page" else 2]
+    before, w = (p.kc.clone(), p.vc.clone()), p.w.clone()
+    kept, lens_out, w_out = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=to)
+    assert mdb._lib.device_status(clear=True) == 2
+    assert bool((kept[0] == -1).all()) and bool((w_out[0] == 0).all()) and lens_out.tolist() == [0, 400]
+    # request 1 alone has moved
+    p.lens = [0, 500]
+    p.check(before, kept, lens_out, w_out, to, 400, 30, w)
+    # a page behind the keys that are written, or of another request that is not read, is nobody's business
+    wide = torch.cat([p.more, p.table[:, :1]], 1)
+    p.lens = [700, 500]
+    p.kc.copy_(before[0]), p.vc.copy_(before[1])
+    kept, lens_out, w_out = mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 400, 30, out_table=wide)
+    p.check(before, kept, lens_out, w_out, wide, 400, 30, w)
+
+
 def test_evict_one_request_to_its_own_row(mdb):
     """A row stride says nothing of a single row."""
     p = Pool([700], 2, 64, BF, seed=43)
