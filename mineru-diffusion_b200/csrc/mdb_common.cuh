@@ -244,6 +244,25 @@ __device__ __forceinline__ float gumbel_noise(uint32_t seed, uint32_t step, uint
 
 static inline bool mdb_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether n x m pieces of `width` neighbouring elements, `row` and `col` elements apart, have no element in common.
+static inline bool mdb_pieces_apart(int64_t n, int64_t row, int64_t m, int64_t col, int64_t width) {
+  typedef __int128 wide;
+  if (n > 1 && row < width && row > -width) return false;
+  if (m > 1 && col < width && col > -width) return false;
+  if (n <= 1 || m <= 1) return true;
+  const wide r = row < 0 ? -static_cast<wide>(row) : row, c = col < 0 ? -static_cast<wide>(col) : col;
+  if (r >= c * (m - 1) + width || c >= r * (n - 1) + width) return true;      // one lies inside the other's steps
+  if (m > n) return mdb_pieces_apart(m, col, n, row, width);
+  for (int64_t j = 1; j < m; ++j) {                        // the multiple of row next to j * col, on either side
+    const wide q = j * c / r;
+    for (wide i = q; i <= q + 1; ++i) {
+      const wide off = j * c - i * r;
+      if (i < n && off < width && off > -static_cast<wide>(width)) return false;
+    }
+  }
+  return true;
+}
+
 // process-wide options (mdb_set_option)
 static int g_opt_pdl = 1;             // programmatic dependent launch between the library's kernels
 static int g_opt_wait_limit_us = 2000000;   // bound of in-kernel waits (mirrors g_wait_limit_ns on the device)

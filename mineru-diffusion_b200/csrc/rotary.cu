@@ -196,9 +196,10 @@ extern "C" int mdb_rotary_embed(const mdb_rotary_embed_args* args, mdb_stream_t 
   MDB_REQUIRE(a.q && a.q_out && a.positions && (a.rot_dims == 0 || a.inv_freq), MDB_ERR_ARG);
   if (a.slots != nullptr) MDB_REQUIRE(a.kv_heads > 0 && a.k && a.k_cache && (!a.v || a.v_cache) && a.num_slots > 0, MDB_ERR_ARG);
   else MDB_REQUIRE((a.kv_heads == 0 || (a.k && a.k_out)) && a.v == nullptr, MDB_ERR_ARG);
-  // (rows of an output that lie on one another)
-  MDB_REQUIRE((a.n == 1 || a.q_out_row != 0) && (a.heads == 1 || a.q_out_head != 0), MDB_ERR_ARG);
-  if (a.slots == nullptr && a.kv_heads > 0) MDB_REQUIRE((a.n == 1 || a.k_out_row != 0) && (a.kv_heads == 1 || a.k_out_head != 0), MDB_ERR_ARG);
-  MDB_REQUIRE(a.dim <= 1024 && static_cast<int64_t>(a.heads) + 2 * static_cast<int64_t>(a.kv_heads) <= 65536, MDB_ERR_UNSUPPORTED);
+  MDB_REQUIRE(a.dim <= 1024 && a.heads <= 65536 && a.kv_heads <= 65536, MDB_ERR_UNSUPPORTED);
+  // heads of an output that lie on one another
+  MDB_REQUIRE(mdb_pieces_apart(a.n, a.q_out_row, a.heads, a.q_out_head, a.dim), MDB_ERR_ARG);
+  if (a.slots == nullptr && a.kv_heads > 0) MDB_REQUIRE(mdb_pieces_apart(a.n, a.k_out_row, a.kv_heads, a.k_out_head, a.dim), MDB_ERR_ARG);
+  MDB_REQUIRE(static_cast<int64_t>(a.heads) + 2 * static_cast<int64_t>(a.kv_heads) <= 65536, MDB_ERR_UNSUPPORTED);
   return a.dtype == MDB_BF16 ? re_launch<bf16>(a, static_cast<cudaStream_t>(stream)) : re_launch<float>(a, static_cast<cudaStream_t>(stream));
 }

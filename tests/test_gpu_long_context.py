@@ -224,6 +224,28 @@ def test_rotary_refusals(mdb):
     assert empty.shape == (0, 2, 64)
 
 
+def test_rotary_outputs_that_overlap_in_part(mdb):
+    q, p = torch.randn(6, 4, 64, generator=gen(8), device=DEV), torch.arange(6, device=DEV)
+    f, _ = mdb.ops.rope_frequencies(64)
+    room = torch.full((8192,), 3.0, device=DEV)
+    for strides in ((128, 64, 1), (256, 32, 1), (64, 6 * 64 - 8, 1), (63, 1000, 1)):
+        with pytest.raises(mdb._lib.MdbError):
+            mdb.ops.rotary_embed(q, None, p, f, q_out=room.as_strided(q.shape, strides))
+        with pytest.raises(mdb._lib.MdbError):
+            mdb.ops.rotary_embed(q, q, p, f, k_out=room.as_strided(q.shape, strides))
+    assert bool((room == 3.0).all())
+    want, _ = mdb.ops.rotary_embed(q, None, p, f)
+    for strides in ((256, 64, 1), (64, 6 * 64, 1), (300, 65, 1), (128, 192, 1)):      # the last: steps of either among the other's
+        if strides[0] == 128:
+            got = room.as_strided((3, 2, 64), strides)
+            mdb.ops.rotary_embed(q[:3, :2], None, p[:3], f, q_out=got)
+            assert torch.equal(got, want[:3, :2])
+        else:
+            got = room.as_strided(q.shape, strides)
+            mdb.ops.rotary_embed(q, None, p, f, q_out=got)
+            assert torch.equal(got, want)
+
+
 # ----------------------------------------------------------------------------- caches
 def paged(lens, g, extra=2):
     """(shuffled page table, pages in all): `extra` pages belong to nobody."""

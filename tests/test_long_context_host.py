@@ -110,6 +110,33 @@ def test_c_entries_refuse_before_any_launch(built):
         assert rotary(**o) == code, o
 
 
+def test_rotary_outputs_that_lie_on_one_another(built):
+    """Row and head strides against the places they name.  Key heads past the limit: the call ends in a refusal either way."""
+    import random
+    lib, at, r = built._lib.lib(), 64, random.Random(5)
+
+    def refused(n, heads, dim, row, head, kv_heads=40000, k_row=40000 * 4096, k_head=4096):
+        a = built._lib.RotaryEmbedArgs(dtype=1, n=n, heads=heads, kv_heads=kv_heads, dim=dim, q_out_row=row, q_out_head=head, k_out_row=k_row, k_out_head=k_head)
+        for f in ("q", "k", "positions", "q_out", "k_out"):
+            setattr(a, f, at)
+        code = lib.mdb_rotary_embed(ctypes.byref(a), None)
+        assert code in (-1, -3)
+        return code == -1
+
+    seen = set()
+    for _ in range(4000):
+        n, heads, dim = r.randint(1, 7), r.randint(1, 7), r.choice([1, 2, 3, 8])
+        row, head = r.randint(-40, 40), r.randint(-40, 40)
+        places = [row * i + head * j + c for i in range(n) for j in range(heads) for c in range(dim)]
+        apart = len(set(places)) == len(places)
+        assert refused(n, heads, dim, row, head) is not apart, (n, heads, dim, row, head)
+        seen.add(apart)
+    assert seen == {True, False}
+    big = 2 ** 62
+    assert not refused(100, 50, 64, big, 64) and not refused(2 ** 31 - 1, 65536, 1024, 65536 * 1024, 1024) and refused(2 ** 31 - 1, 65536, 1024, 1024, 1024)
+    assert refused(4, 2, 64, 128, 64, k_row=4096 * 39999, k_head=4096) and refused(4, 2, 64, 128, 64, k_row=63, k_head=4096)
+
+
 def test_eviction_with_wide_weights_refused(built):
     lib, at = built._lib.lib(), 64
 
