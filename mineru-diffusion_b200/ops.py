@@ -1097,6 +1097,8 @@ def block_attn_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         room = shared_prefix_workspace_bytes(bs, block, hq, hkv)
         workspace = q.new_empty(room, dtype=torch.uint8)
     else:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         room = workspace.numel() * workspace.element_size()
     args = _pack_shared(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),

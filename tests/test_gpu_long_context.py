@@ -526,6 +526,16 @@ def test_shared_prefix_refusals(mdb):
         f(b.q, b.kc, b.vc, None, None, b.seqlens, b.table, softmax_scale=-1.0)
 
 
+def test_shared_prefix_workspace_of_fewer_places_than_numbers(mdb):
+    """An expanded or strided workspace has not the room that its shape says."""
+    b = Batch([30, 70], 50, 8, 4, 2)
+    need = mdb.ops.shared_prefix_workspace_bytes(2, 8, 4, 2)
+    for room in (torch.empty(16, dtype=torch.uint8, device=DEV).expand(need // 16 + 1, 16), torch.empty(2 * need, dtype=torch.uint8, device=DEV)[::2]):
+        with pytest.raises(ValueError):
+            b.call(mdb, workspace=room)
+    b.check(*b.call(mdb, workspace=torch.empty(need // 8, 8, dtype=torch.uint8, device=DEV)))
+
+
 # ----------------------------------------------------------------------------- weights of the keys
 def check_weights(b, got, lse, previous=None, decay=1.0, scale=D ** -0.5):
     group = b.hq // b.hkv
