@@ -777,11 +777,12 @@ int mdb_key_weights(const mdb_key_weights_args* args, mdb_stream_t stream);
  * in front stay (NaN counts as the lowest weight; the lowest index wins a tie); all of them where there are no more than budget.
  * Their rows of row_bytes bytes (a multiple of 16) in K and V, and their weights, move in order to the first places of the
  * request's pages (out_table NULL, or block_table with its stride) or of the pages in out_table, which hold none of those
- * read: a request that would write a page of its own that it reads keeps nothing (kept -1, weights and length 0, caches as they were),
- * with MDB_STATUS_BAD_PAGE; between requests this is the caller's to keep.  Pages that are written
- * belong to one request.  kept [bs][kv_heads][budget] = old places, -1 behind the last; weights_out (may be NULL, may be
- * weights) gets 0 there, and behind the budget in all of its columns: of these it has weight_cols where it is weights (strides too) and
- * budget otherwise, or as many as mdb_kv_evict_wide is told (at least budget).  seqlens_out (may be seqlens) = min(seqlens, budget). */
+ * read: a request that would write a page of its own that it reads keeps nothing (kept -1, weights and length 0, caches as they
+ * were), with MDB_STATUS_BAD_PAGE; between requests this is the caller's to keep.  Pages that are written belong to one request.
+ * kept [bs][kv_heads][budget] = old places, -1 behind the last; weights_out (may be NULL, may be weights) gets 0 there, and
+ * behind the budget in all of its columns: of these it has weight_cols where it is weights (strides too) and budget otherwise,
+ * or as many as mdb_kv_evict_wide is told (at least budget); its rows have none in common.  seqlens_out (may be seqlens) =
+ * min(seqlens, budget). */
 typedef struct {
   int32_t bs, kv_heads, row_bytes, budget, recent, num_pages, table_stride, table_pages, out_table_stride, out_table_pages;
   void* k_cache;

@@ -333,8 +333,11 @@ extern "C" int mdb_kv_evict_wide(const mdb_kv_evict_args* args, int64_t weight_o
   MDB_REQUIRE(a.k_cache && a.v_cache && a.weights && a.seqlens && a.seqlens_out && a.block_table && a.kept, MDB_ERR_ARG);
   MDB_REQUIRE(a.out_table == nullptr || (a.out_table_pages > 0 && (a.out_table_stride >= a.out_table_pages || a.bs <= 1)), MDB_ERR_ARG);
   MDB_REQUIRE(a.row_bytes % 16 == 0 && mdb_aligned16(a.k_cache) && mdb_aligned16(a.v_cache), MDB_ERR_ALIGN);
-  MDB_REQUIRE(static_cast<int64_t>(a.bs) * a.kv_heads <= 32767 && a.row_bytes <= 4096 && a.budget <= (1 << 23) && a.table_pages <= (1 << 22) && a.out_table_pages <= (1 << 22),
+  MDB_REQUIRE(static_cast<int64_t>(a.bs) * a.kv_heads <= 32767 && a.budget <= (1 << 23) && a.table_pages <= (1 << 22) && a.out_table_pages <= (1 << 22),
               MDB_ERR_UNSUPPORTED);
+  // rows of weights that lie on one another
+  MDB_REQUIRE(a.weights_out == nullptr || mdb_pieces_apart(a.bs, a.weight_out_row, a.kv_heads, a.weight_out_head, weight_out_cols), MDB_ERR_ARG);
+  MDB_REQUIRE(a.row_bytes <= 4096, MDB_ERR_UNSUPPORTED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int pairs = a.bs * a.kv_heads;
   // the same table once more: in place (a table that starts at the same entry with rows further apart is another one)

@@ -892,6 +892,15 @@ def test_evict_leaves_no_weight_behind_the_last_key(mdb, lens, budget, recent):
     assert bool((beside[..., cols + 7:] == 5.0).all())
 
 
+def test_evict_weights_of_one_row_for_all(mdb):
+    p = Pool([300, 90], 2, 64, BF, seed=45)
+    before = p.kc.clone()
+    for room in (torch.zeros(1, 2, 100, device=DEV).expand(2, -1, -1), torch.zeros(2, 1, 100, device=DEV).expand(-1, 2, -1)):
+        with pytest.raises(mdb._lib.MdbError):
+            mdb.ops.evict_kvcache(p.kc, p.vc, p.w, p.seqlens, p.table, 100, weights_out=room)
+    assert torch.equal(p.kc, before)
+
+
 def test_weights_of_keys_that_follow_an_eviction(mdb):
     """One buffer of weights for a request that shrinks and grows again."""
     b = Batch([500, 90], 0, 8, 4, 2, seed=40)

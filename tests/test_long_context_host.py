@@ -152,6 +152,22 @@ def test_eviction_with_wide_weights_refused(built):
     assert wide(9) == -1 and wide(0) == -1 and wide(100, row_bytes=24) == -2 and wide(0, weights_out=None, row_bytes=24) == -2
 
 
+def test_eviction_to_weights_that_lie_on_one_another(built):
+    lib, at = built._lib.lib(), 64
+
+    def code(bs, row, head, cols):      # rows of 8192 bytes: refused either way
+        a = built._lib.KvEvictArgs(bs=bs, kv_heads=3, row_bytes=8192, budget=10, recent=2, num_pages=4, table_stride=2, table_pages=2, weight_cols=100,
+                                   weight_out_row=row, weight_out_head=head)
+        for n in ("k_cache", "v_cache", "weights", "weights_out", "seqlens", "seqlens_out", "block_table", "kept"):
+            setattr(a, n, at)
+        return lib.mdb_kv_evict_wide(ctypes.byref(a), cols, None)
+
+    for bs, row, head, cols in ((1, 0, 10, 10), (1, 0, 12, 12), (4, 30, 10, 10), (4, 10, 40, 10), (4, 37, 12, 11)):
+        assert code(bs, row, head, cols) == -3
+    for bs, row, head, cols in ((1, 0, 10, 11), (1, 0, 0, 10), (4, 30, 10, 11), (4, 29, 10, 10), (4, 10, 0, 10), (4, 0, 10, 10), (2, 5, 100, 10)):
+        assert code(bs, row, head, cols) == -1
+
+
 def test_workspace_of_the_shared_prefix(built):
     need = built.ops.shared_prefix_workspace_bytes
     assert need(0, 32, 16, 8) == 0 and need(4, 32, 16, 5) == 0
