@@ -703,6 +703,28 @@ static bool get_q_tensor_map(const void* ptr, int64_t tokens, int64_t row_stride
   return true;
 }
 
+// The same maps for calls whose addresses do not come back: encoded anew every time (about a microsecond, on the host).
+static bool encode_map(const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMap* out) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return enc != nullptr && enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// q [tokens][hq][128] in boxes of 64 channels x group heads x box_tokens tokens
+static bool encode_queries(const void* q, int64_t tokens, int hq, int group, int box_tokens, CUtensorMap* out) {
+  const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(hq), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(hq) * kHeadDim * 2};
+  const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_tokens)};
+  return encode_map(q, 3, dims, strides, box, out);
+}
+// a cache as [pages * 256][hkv * 128] in boxes of 64 channels x 128 keys
+static bool encode_cache(const void* cache, int num_pages, int hkv, CUtensorMap* out) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(hkv) * kHeadDim, static_cast<cuuint64_t>(num_pages) * kPage};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(hkv) * kHeadDim * 2};
+  const cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(kAtKeys)};
+  return encode_map(cache, 2, dims, strides, box, out);
+}
+
 static int at_sm_count() {
   static int sm_count = 0;
   if (sm_count == 0) {

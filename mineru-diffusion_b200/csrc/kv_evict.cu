@@ -350,7 +350,7 @@ extern "C" int mdb_kv_evict_wide(const mdb_kv_evict_args* args, int64_t weight_o
   int slice = 1;
   while (slice < 32 && pieces % (2 * slice) == 0) slice *= 2;
   if (!apart) {
-    while (slice > 2 && static_cast<int64_t>(pairs) * 2 * (pieces / slice) < 2 * 148) slice /= 2;
+    while (slice > 2 && static_cast<int64_t>(pairs) * 2 * (pieces / slice) < 2 * at_sm_count()) slice /= 2;
     return mdb_launch(evict_move_kernel<true>, dim3(2 * pairs * (pieces / slice)), dim3(kEvMoveThreads), 0, st, a, slice);
   }
   return mdb_launch(evict_move_kernel<false>, dim3(2 * pairs * (pieces / slice), (a.budget + kEvMoveRows - 1) / kEvMoveRows), dim3(kEvMoveThreads), 0, st, a,

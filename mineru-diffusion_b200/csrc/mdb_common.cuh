@@ -173,6 +173,11 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // The three bf16 parts of a pair of numbers: 24 significant bits are the exact sum of three times eight, cut and not rounded (the
 // upper half of x, that of what is left, the rest).  The second comes times 2^6, the third times 2^12, as no bf16 number is below 2^-133:
 // numbers from 2^-122 on are taken apart exactly, smaller ones to 2^-145.  (No larger factor: sums of products of first and

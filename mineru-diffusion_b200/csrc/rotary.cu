@@ -171,7 +171,7 @@ static int re_launch(const mdb_rotary_embed_args& a, cudaStream_t st) {
   // turns of about as many columns each, whole warps
   const int turns = (columns + kReThreads - 1) / kReThreads, threads = ((columns + turns - 1) / turns + 31) / 32 * 32;
   // a token per CTA while all CTAs are resident at once (48 registers a thread), then as few full rounds as there can be
-  const int64_t resident = 148 * (65536 / (48 * threads)), rounds = (a.n + resident * kReTokens - 1) / (resident * kReTokens);
+  const int64_t resident = at_sm_count() * static_cast<int64_t>(65536 / (48 * threads)), rounds = (a.n + resident * kReTokens - 1) / (resident * kReTokens);
   int tokens = static_cast<int>((a.n + resident * rounds - 1) / (resident * rounds));
   while (tokens > 1 && sizeof(float2) * tokens * (a.rot_dims / 2) > 40 * 1024) tokens /= 2;
   const dim3 grid((a.n + tokens - 1) / tokens), block(threads);
