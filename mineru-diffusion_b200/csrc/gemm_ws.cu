@@ -530,7 +530,23 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// An encode call of the driver needs the thread's context, which a thread gets with its first call of the runtime that works on the device:
+// where it has made none yet, here.
+static void bind_context() {
+  typedef CUresult (*GetCurrentFn)(CUcontext*);
+  static const GetCurrentFn get_current = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool found = cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<GetCurrentFn>(p) : static_cast<GetCurrentFn>(nullptr);
+  }();
+  CUcontext context = nullptr;
+  int dev = 0;
+  if (get_current != nullptr && get_current(&context) == CUDA_SUCCESS && context == nullptr && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+}
+
 static EncodeTiledFn encode_tiled_fn() {
+  bind_context();
   static EncodeTiledFn fn = nullptr;
   static bool tried = false;
   if (!tried) {

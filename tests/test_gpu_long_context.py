@@ -993,3 +993,35 @@ def test_two_streams_at_once(mdb):
     for b, out, lse, w in got:
         b.check(out, lse)
         check_weights(b, w, lse)
+
+
+def test_first_call_of_a_thread(mdb):
+    """A thread that has not touched the device yet: the calls that describe their operands to the driver bring it up themselves."""
+    import threading
+    b = Batch([300], 40, 4, 4, 2, seed=61)
+    out, lse = b.call(mdb)
+    weights = mdb.ops.key_weights(b.q, b.kc, lse, b.seqlens, b.table)
+    plain = mdb.ops.block_attn_with_kvcache(b.q, b.kc, b.vc, b.seqlens, b.table)
+    x, w = torch.randn(32, 256, generator=gen(62), device=DEV).to(BF), torch.randn(512, 256, generator=gen(63), device=DEV).to(BF)
+    product = mdb.ops.linear(x, w)
+    room, room_q, room_w = torch.empty(1, 2, b.table.shape[1] * PAGE, device=DEV), torch.empty_like(b.q), torch.empty_like(product)
+    # addresses that no call has seen
+    q, xs, kc, vc = b.q.clone(), x.clone(), b.kc.clone(), b.vc.clone()
+    scratch = torch.empty(mdb.ops.shared_prefix_workspace_bytes(1, 4, 4, 2), dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    for f, want in ((lambda: mdb.ops.key_weights(q, kc, lse, b.seqlens, b.table, out=room), weights),
+                    (lambda: mdb.ops.block_attn_shared_prefix(q, kc, vc, b.prefix_len, b.prefix_table, b.seqlens, b.table, out=room_q, workspace=scratch), out),
+                    (lambda: mdb.ops.block_attn_with_kvcache(q, kc, vc, b.seqlens, b.table, out=room_q), plain), (lambda: mdb.ops.linear(xs, w, out=room_w), product)):
+        got = []
+
+        def call():
+            try:
+                got.append(f())
+            except Exception as e:
+                got.append(e)
+
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+        assert torch.is_tensor(got[0]), got[0]
+        assert torch.equal(got[0], want)
