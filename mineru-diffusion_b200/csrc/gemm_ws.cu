@@ -530,33 +530,28 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// An entry of the driver, NULL if there is none; where it is kept in a static, threads that come while it is looked up wait for it.
+template <typename Fn>
+static Fn driver_entry(const char* name) {
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  const bool found = cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+  return found ? reinterpret_cast<Fn>(p) : static_cast<Fn>(nullptr);
+}
+
 // An encode call of the driver needs the thread's context, which a thread gets with its first call of the runtime that works on the device:
 // where it has made none yet, here.
 static void bind_context() {
   typedef CUresult (*GetCurrentFn)(CUcontext*);
-  static const GetCurrentFn get_current = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    const bool found = cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
-    return found ? reinterpret_cast<GetCurrentFn>(p) : static_cast<GetCurrentFn>(nullptr);
-  }();
+  static const GetCurrentFn get_current = driver_entry<GetCurrentFn>("cuCtxGetCurrent");
   CUcontext context = nullptr;
   int dev = 0;
   if (get_current != nullptr && get_current(&context) == CUDA_SUCCESS && context == nullptr && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
 }
 
 static EncodeTiledFn encode_tiled_fn() {
+  static const EncodeTiledFn fn = driver_entry<EncodeTiledFn>("cuTensorMapEncodeTiled");
   bind_context();
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
   return fn;
 }
 

@@ -1025,3 +1025,37 @@ def test_first_call_of_a_thread(mdb):
         t.join()
         assert torch.is_tensor(got[0]), got[0]
         assert torch.equal(got[0], want)
+
+
+FIRST_CALLS = """
+import importlib, sys, threading
+import torch
+sys.path.insert(0, {root!r})
+mdb = importlib.import_module("mineru-diffusion_b200")
+q, kc = torch.randn(1, 4, 4, 128, device="cuda").bfloat16(), torch.randn(2, 256, 2, 128, device="cuda").bfloat16()
+lse, n, table = torch.zeros(1, 4, 4, device="cuda"), torch.tensor([300], dtype=torch.int32, device="cuda"), torch.tensor([[1, 0]], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+at_once, got = threading.Barrier(24), []
+def call():
+    at_once.wait()
+    try:
+        got.append(mdb.ops.key_weights(q, kc, lse, n, table))
+    except Exception as e:
+        got.append(e)
+threads = [threading.Thread(target=call) for _ in range(24)]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+wrong = [x for x in got if not torch.is_tensor(x) or not torch.equal(x, got[0])]
+assert len(got) == 24 and torch.is_tensor(got[0]) and not wrong, wrong
+"""
+
+
+def test_first_calls_of_many_threads_at_once():
+    """In a process of its own: what the library looks up once is there for every thread that asks at the same time."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    for _ in range(3):
+        done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=ROOT)], capture_output=True, text=True, timeout=300)
+        assert done.returncode == 0, done.stderr[-2000:]
