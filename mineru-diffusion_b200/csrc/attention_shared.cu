@@ -695,11 +695,9 @@ __global__ void __launch_bounds__(256) attn_shared_merge(const ShArgs a) {
     if (len[own] == 0) continue;
     if (!sh_info_there(more[own].x, more[own].y, a.ctas)) {
       // the unit has no parts: its row is not a number
-      l = __int_as_float(0x7fffffff);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = make_float4(l, l, l, l);
+      more[own].y = 0;
+      first_ml[own] = make_float2(0.f, __int_as_float(0x7fffffff));
       if (quad == 0) report_status(MDB_STATUS_WAIT_TIMEOUT);
-      break;
     }
     join(first_ml[own], first[own]);
     for (int c0 = 1; c0 <= more[own].y; c0 += kShJoin) {   // several in flight

@@ -256,7 +256,12 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             float x[32];
             tmem_ld32(tmem_base + wg * kKwMaxRows + lane_field + c, x);      // (columns behind the last row are not looked at)
             tmem_ld_wait();
-            if (c + 32 <= rows && !none) {
+            if (none) {                // (apart: as a condition of every exponential it costs 2 %, eight rows to a key head)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (neg_lse[c + i] == -INFINITY) x[i] = 0.f;
+            }
+            if (c + 32 <= rows) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float4 n = *reinterpret_cast<const float4*>(neg_lse + c + i);
@@ -268,7 +273,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             } else {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (c + i < rows && neg_lse[c + i] != -INFINITY) acc += ex2_approx(fmaf(x[i], a.scale_log2, neg_lse[c + i]));
+                if (c + i < rows) acc += ex2_approx(fmaf(x[i], a.scale_log2, neg_lse[c + i]));
             }
           }
           tc_fence_before();
