@@ -735,7 +735,8 @@ int mdb_rotary_embed(const mdb_rotary_embed_args* args, mdb_stream_t stream);
 /* Block attention of a batch whose requests share a prefix: as mdb_attn_block_paged, but every query row sees the prefix_len[0]
  * keys of the pages in prefix_table (once, for all requests) and then keys [0, ctx_lens[b]) of its request's own pages.
  * lse (may be NULL) [bs][block][hq] = the natural logarithm of the softmax's denominator.  A row without any key gets zeros and
- * -inf.  prefix_pages 0: no prefix (prefix_table and prefix_len may be NULL).  The workspace is always needed; calls in flight at
+ * -inf.  For few requests or a short prefix (see csrc/attention_shared.cu) mdb_attn_block_paged over joined tables is the faster
+ * call.  prefix_pages 0: no prefix (prefix_table and prefix_len may be NULL).  The workspace is always needed; calls in flight at
  * the same time need one each. */
 int64_t mdb_attn_shared_workspace_bytes(int bs, int block, int hq, int hkv);
 typedef struct {

@@ -13,9 +13,12 @@
 // groups of four warps that take the tiles in turn.  More than 128 rows per key head go in blocks of rows over up to 16 tiles at
 // a time, sums in shared memory.
 //
-// Bound by memory (256 bytes per key and head) up to 64 rows: 32 requests of 4096 to 8192 keys, eight heads, 73 us = 5.7 TB/s; 128 rows 89 us,
-// 256 (twice over the keys) 86 for half the requests: exponentials, 16 a clock and SM.  Two groups of warps instead of four: 78, 100, 81 us.
-// The loop over a tile's rows is kept short: with the next scores asked for ahead, in two copies of it, 83 for 78 us.
+// Bound by memory (256 bytes per key and head) up to 64 rows: 32 requests of 4096 to 8192 keys, eight heads, 73 us = 5.8 TB/s in a graph (77 in a
+// long loop, at the power limit); 128 rows 82 us, 256 (twice over the keys) 76 for half the requests: exponentials, 16 a clock and SM.
+// The loop over a tile's rows is kept short: with the next scores asked for ahead, in two copies of it, 5 us longer.
+// A prefix's keys with the rows of a batch, 16 query and 8 key heads: 128 tokens 17 us behind 16384 keys; 1024 tokens 36 behind 1056 and 99
+// behind 16384, 2048 tokens 67 and 195 (exponentials alone 4, 60, 8 and 119).  A CTA with a single tile takes all its blocks of rows through one
+// group of warps, and K is loaded anew for each.
 #include "mdb_common.cuh"
 
 namespace mdb {

@@ -12,9 +12,10 @@
 //                         new place is never behind its old one, so a CTA that has a slice of the channels of all rows walks
 //                         them in order, loads of a step in front of its stores.
 //
-// Bound by memory: rows read and written once.  16 requests of 16384 to 32768 keys, eight heads, 8192 stay: 166 us = 6.4 TB/s for the
-// rows (places looked up by every piece, heads one behind the other: 297), 23 us for the selection in front of them (31 before its
-// weights stayed in registers).
+// Bound by memory: rows read and written once.  16 requests of 16384 to 32768 keys, eight heads, 8192 stay: 170 us = 6.3 TB/s for the
+// rows (places looked up by every piece, heads one behind the other: 297), 22 us for the selection in front of them (31 before its
+// weights stayed in registers); 189 together.  In place 16 requests of 32768 keys take 225 us and one of 30000 that keeps 8000 takes 48
+// (20 of them the selection, with a CTA per key head) for 10 of reading and writing: a CTA walks its slice alone, a step at a time.
 #include "mdb_common.cuh"
 
 namespace mdb {

@@ -1066,7 +1066,9 @@ def block_attn_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                              out: torch.Tensor | None = None, want_lse: bool = False, lse: torch.Tensor | None = None):
     """``block_attn_with_kvcache`` for a batch whose requests share a prefix: every query of q [bs, B, Hq, 128] sees the
     ``prefix_seqlen`` (int32 [1]) keys of the pages ``prefix_table`` (int32 [pages]) and then the ``cache_seqlens[b]`` keys of its
-    request's pages.  The prefix is read and multiplied once for all requests.  None, None: no prefix.  A row that sees no key
+    request's pages.  The prefix is read and multiplied once for all requests, which pays from about 16384 (requests x prefix keys) on
+    with single tokens and from about 65536 on with blocks of 32; below that ``block_attn_with_kvcache`` over tables that begin
+    with the prefix's pages (of whole pages) is the faster call, where lse is not wanted.  None, None: no prefix.  A row that sees no key
     gets zeros.  Returns out, or (out, lse) with ``want_lse`` or ``lse`` (fp32 [bs, B, Hq], the logarithm of the softmax's
     denominator, -inf where there is no key): what ``key_weights`` takes.  Calls in flight at the same time need a ``workspace``
     (``shared_prefix_workspace_bytes``) each."""
