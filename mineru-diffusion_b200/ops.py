@@ -47,6 +47,15 @@ def _rows(t: torch.Tensor, name: str) -> int:
     return t.stride(0)
 
 
+def _room(workspace: torch.Tensor | None) -> int:
+    """Bytes of a workspace (None: 0).  One that is not contiguous has not the room that its shape says."""
+    if workspace is None:
+        return 0
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return workspace.numel() * workspace.element_size()
+
+
 OPT_PDL = 1             # programmatic dependent launch between kernels (default on)
 OPT_GEMM_PAIR = 3       # many-row GEMMs on CTA pairs (tcgen05.mma.cta_group::2): 1 from 2048 rows (default), 2 from 256, 0 never
 OPT_WAIT_LIMIT_US = 4   # bound of every in-kernel wait in microseconds (default 2 s); expiry raises status bit 16
@@ -155,9 +164,9 @@ def block_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if out is None:
         out = torch.empty_like(q)
     need = _lib.lib().mdb_attn_paged_workspace_bytes(bs, block, hq, nsplit)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    ws_bytes = _room(workspace)
+    if ws_bytes < need:
+        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
     _lib.check(_lib.lib().mdb_attn_block_paged(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
                                                block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(),
                                                bs, block, hq, hkv, pages, float(softmax_scale), nsplit,
@@ -400,8 +409,9 @@ def lm_head_sample(hidden: torch.Tensor, weight: torch.Tensor, temperatures: tor
         if tuple(noise.shape) != (m, vocab) or not noise.is_contiguous():
             raise ValueError("noise must be a contiguous [m, vocab] tensor")
     need = lmhead_workspace_bytes(m, vocab)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=hidden.device)
+    room = _room(workspace)
+    if workspace is None or room < need:
+        workspace, room = torch.empty(need, dtype=torch.uint8, device=hidden.device), need
     if x0 is None:
         x0 = torch.empty(m, dtype=torch.int32, device=hidden.device)
     if conf is None:
@@ -409,8 +419,7 @@ def lm_head_sample(hidden: torch.Tensor, weight: torch.Tensor, temperatures: tor
     _lib.check(_lib.lib().mdb_lmhead_sample(hidden.data_ptr(), _rows(hidden, "hidden"), weight.data_ptr(), m, vocab, h,
                                             temperatures.data_ptr(), block, mode, _ptr(noise), int(seed or 0) & 0xFFFFFFFF,
                                             int(step) & 0xFFFFFFFF, _ptr(step_dev), workspace.data_ptr(),
-                                            workspace.numel() * workspace.element_size(), x0.data_ptr(),
-                                            conf.data_ptr(), _stream()), "mdb_lmhead_sample")
+                                            room, x0.data_ptr(), conf.data_ptr(), _stream()), "mdb_lmhead_sample")
     return x0, conf
 
 
@@ -544,7 +553,7 @@ def lm_head_sample_tp(hidden: torch.Tensor, weight: torch.Tensor, temperatures: 
                                                h, temperatures.data_ptr(), block, mode, _ptr(noise),
                                                int(seed or 0) & 0xFFFFFFFF, int(step) & 0xFFFFFFFF, _ptr(step_dev),
                                                workspace.data_ptr(), peer_workspace_ptr,
-                                               workspace.numel() * workspace.element_size(), tile_begin, tile_count,
+                                               _room(workspace), tile_begin, tile_count,
                                                peer_flags_ptr, wait_flags_ptr, wait_count, tag, epoch.data_ptr(),
                                                x0.data_ptr(), conf.data_ptr(), _stream()), "mdb_lmhead_sample_tp")
     return x0, conf
@@ -832,7 +841,7 @@ def latent_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
     _lib.check(_lib.lib().mdb_latent_attn(
         _act_dtype(q, "q"), q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), block_table.stride(0),
         row_seq.data_ptr(), row_pos.data_ptr(), m, heads, width, cache.shape[0] // 256, scale, nsplit, _ptr(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()), "mdb_latent_attn")
+        _room(workspace), _stream()), "mdb_latent_attn")
 
 
 def gather_latents(cache: torch.Tensor, block_table: torch.Tensor, cu: torch.Tensor, nseq: int, out: torch.Tensor) -> None:
@@ -887,7 +896,7 @@ def window_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
         v_cache=v_cache.data_ptr(), block_table=block_table.data_ptr(), row_seq=row_seq.data_ptr(), row_pos=row_pos.data_ptr(),
         cu_q=cu_q.data_ptr(), start=start.data_ptr(), table_stride=block_table.stride(0), num_pages=k_cache.shape[0] // 256,
         gate=_rows_c(gate), out=out.data_ptr(), ld_out=_rows(out, "out"), workspace=_ptr(workspace),
-        workspace_bytes=0 if workspace is None else workspace.numel() * workspace.element_size())
+        workspace_bytes=_room(workspace))
     _lib.check(_lib.lib().mdb_window_attn(a, _stream()), "mdb_window_attn")
 
 
@@ -1099,9 +1108,7 @@ def block_attn_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         room = shared_prefix_workspace_bytes(bs, block, hq, hkv)
         workspace = q.new_empty(room, dtype=torch.uint8)
     else:
-        if not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous")
-        room = workspace.numel() * workspace.element_size()
+        room = _room(workspace)
     args = _pack_shared(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
         0 if prefix_table is None else prefix_table.data_ptr(), 0 if prefix_seqlen is None else prefix_seqlen.data_ptr(), block_table.data_ptr(),

@@ -536,6 +536,16 @@ def test_shared_prefix_workspace_of_fewer_places_than_numbers(mdb):
     b.check(*b.call(mdb, workspace=torch.empty(need // 8, 8, dtype=torch.uint8, device=DEV)))
 
 
+def test_block_attention_workspace_of_fewer_places_than_numbers(mdb):
+    b = Batch([900, 70], 0, 8, 4, 2, seed=64)
+    need = mdb.ops.attn_workspace_bytes(2, 8, 4, 3)
+    want = mdb.ops.block_attn_with_kvcache(b.q, b.kc, b.vc, b.seqlens, b.table, nsplit=3)
+    with pytest.raises(ValueError):
+        mdb.ops.block_attn_with_kvcache(b.q, b.kc, b.vc, b.seqlens, b.table, nsplit=3, workspace=torch.empty(16, dtype=torch.uint8, device=DEV).expand(need // 16 + 1, 16))
+    for room in (None, torch.empty(need, dtype=torch.uint8, device=DEV), torch.empty(16, dtype=torch.uint8, device=DEV)):      # (too small: one is allocated)
+        assert torch.equal(mdb.ops.block_attn_with_kvcache(b.q, b.kc, b.vc, b.seqlens, b.table, nsplit=3, workspace=room), want)
+
+
 # ----------------------------------------------------------------------------- weights of the keys
 def check_weights(b, got, lse, previous=None, decay=1.0, scale=D ** -0.5):
     group = b.hq // b.hkv

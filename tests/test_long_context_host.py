@@ -176,6 +176,15 @@ def test_workspace_of_the_shared_prefix(built):
     assert need(8, 32, 16, 8) > need(4, 32, 16, 8)
 
 
+def test_room_of_a_workspace(built):
+    room = built.ops._room
+    x = torch.empty(6, 8)
+    assert room(None) == 0 and room(x) == 192 and room(x[2:]) == 128 and room(x[0:0]) == 0 and room(x[:, :1].contiguous()) == 24
+    for bad in (x[:1].expand(100, 8), x[:, ::2], x.t(), torch.empty(1, dtype=torch.uint8).expand(1 << 30)):
+        with pytest.raises(ValueError):
+            room(bad)
+
+
 def test_wrappers_refuse_cpu_tensors(built):
     x = torch.zeros(2, 1, 64)
     with pytest.raises(RuntimeError):
