@@ -168,6 +168,13 @@ def test_eviction_to_weights_that_lie_on_one_another(built):
         assert code(bs, row, head, cols) == -1
 
 
+def test_argument_blocks_keep_their_size(built):
+    """Callers built against an earlier header pass blocks of these sizes; what came later (mdb_kv_evict_wide) is an argument of its own."""
+    sizes = {'RotaryEmbedArgs': 208, 'AttnSharedArgs': 128, 'KeyWeightsArgs': 104, 'KvEvictArgs': 152}
+    for name, size in sizes.items():
+        assert ctypes.sizeof(getattr(built._lib, name)) == size, name
+
+
 def test_workspace_of_the_shared_prefix(built):
     need = built.ops.shared_prefix_workspace_bytes
     assert need(0, 32, 16, 8) == 0 and need(4, 32, 16, 5) == 0
