@@ -710,9 +710,9 @@ int mdb_pick_token(const float* logits, int64_t ld, int m, int vocab, const floa
 /* Rotary positions without a norm: with t = positions[row] * inv_freq[i] the channel pair (i, i + rot_dims / 2) of a head, or
  * with `interleaved` (2 i, 2 i + 1), becomes scale * (a cos t - b sin t, b cos t + a sin t); `inverse` turns by -t (the
  * gradient with respect to the input is the inverse turn of the gradient).  Channels from rot_dims on pass as they come.  Rows
- * and heads lie *_row and *_head elements apart, those of an output without one in common; outputs may be the inputs.  With slots (int32 [n], -1: skipped) the keys, and
- * the values v as they come (NULL: none), go to rows of the contiguous caches [num_slots][kv_heads][dim] and k_out is
- * not used; without slots v must be NULL.  kv_heads 0: queries alone. */
+ * and heads lie *_row and *_head elements apart, those of an output without one in common; outputs may be the inputs.  With
+ * slots (int32 [n], -1: skipped) the keys, and the values v as they come (NULL: none), go to rows of the contiguous caches
+ * [num_slots][kv_heads][dim] and k_out is not used; without slots v must be NULL.  kv_heads 0: queries alone. */
 typedef struct {
   int32_t dtype, n, heads, kv_heads, dim, rot_dims, interleaved, inverse;
   const void* q;
