@@ -1004,6 +1004,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise ValueError("inv_freq must be a contiguous float64 vector of at most half as many entries as a head has channels")
     if q_out is None:
         q_out = torch.empty_like(q)              # (of a view of a wider tensor: contiguous)
+        if q_out.stride(2) != 1:                 # (of rows that overlap: channels need not be dense)
+            q_out = q.new_empty(q.shape)
     _, qo_row, qo_head = _heads_strides(q_out, n, d, dtype, "q_out", hq)
     hkv, k_row, k_head = (0, 0, 0) if k is None else _heads_strides(k, n, d, dtype, "k")
     v_row = v_head = ko_row = ko_head = slots = 0

@@ -224,6 +224,17 @@ def test_rotary_refusals(mdb):
     assert empty.shape == (0, 2, 64)
 
 
+def test_rotary_of_rows_that_overlap(mdb):
+    """Windows of one vector: inputs may share elements, the output that is made for them does not."""
+    x, f = torch.randn(400, generator=gen(9), device=DEV), mdb.ops.rope_frequencies(8)[0]
+    for shape, strides in (((2, 2, 8), (1, 8, 1)), ((5, 3, 8), (3, 8, 1)), ((4, 3, 8), (8, 1, 1)), ((3, 2, 8), (0, 0, 1))):
+        q, p = x.as_strided(shape, strides), torch.arange(shape[0], device=DEV) * 11
+        got, _ = mdb.ops.rotary_embed(q, None, p, f)
+        check_turn(got, q, p, f, False)
+        _, got = mdb.ops.rotary_embed(q, q, p, f)
+        check_turn(got, q, p, f, False)
+
+
 def test_rotary_outputs_that_overlap_in_part(mdb):
     q, p = torch.randn(6, 4, 64, generator=gen(8), device=DEV), torch.arange(6, device=DEV)
     f, _ = mdb.ops.rope_frequencies(64)
